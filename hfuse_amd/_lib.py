@@ -17,6 +17,8 @@ HF_BARRIER_NONE, HF_BARRIER_MATCHED, HF_BARRIER_SUBSET, HF_BARRIER_BLOCKIDX = 0,
 HF_SPLIT_TABLE, HF_SPLIT_EXECTIME = -1, -2
 HF_STREAM_EMPTY, HF_STREAM_READ, HF_STREAM_WRITE, HF_STREAM_READ_LINES, HF_STREAM_COPY_1_4 = 0, 1, 2, 3, 4
 HF_STREAM_WRITE_STRIDED, HF_STREAM_WRITE_XCD = 5, 6
+HF_F32, HF_BF16, HF_F16 = 0, 1, 2
+HF_I32, HF_I64 = 0, 1
 ABI_VERSION = 300          # what hf_version() of a matching library answers
 HF_MAX_SEARCH_RESULTS = 64
 HF_MAX_TENSORINFO_DIMS = 8
@@ -132,6 +134,31 @@ class Blake2bArgs(C.Structure):
                 ("target2", C.c_uint32 * 2)]
 
 
+class LayerNormArgs(C.Structure):
+    _fields_ = [(k, C.c_void_p) for k in ("x", "weight", "bias", "y", "mean", "rstd")] + \
+               [(k, C.c_int64) for k in ("rows", "cols", "x_stride", "y_stride")] + \
+               [("eps", C.c_float), ("type", C.c_int), ("param_type", C.c_int)]
+
+
+class LayerNormBackwardArgs(C.Structure):
+    _fields_ = [(k, C.c_void_p) for k in ("dy", "x", "weight", "mean", "rstd", "dx", "dweight", "dbias")] + \
+               [(k, C.c_int64) for k in ("rows", "cols", "dy_stride", "x_stride", "dx_stride")] + \
+               [("type", C.c_int), ("param_type", C.c_int), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class EmbeddingArgs(C.Structure):
+    _fields_ = [(k, C.c_void_p) for k in ("tokens", "weight", "out")] + \
+               [(k, C.c_int64) for k in ("ntokens", "vocab", "cols", "weight_stride", "out_stride")] + \
+               [("scale", C.c_float), ("type", C.c_int), ("index_type", C.c_int)]
+
+
+class EmbeddingBackwardArgs(C.Structure):
+    _fields_ = [(k, C.c_void_p) for k in ("dy", "tokens", "dweight")] + \
+               [(k, C.c_int64) for k in ("ntokens", "vocab", "cols", "dy_stride", "dweight_stride", "padding_idx")] + \
+               [("scale", C.c_float), ("type", C.c_int), ("out_type", C.c_int), ("index_type", C.c_int),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 # every symbol include/hfuse_gfx950.h declares, with its prototype
 PROTOTYPES = {
     "hf_last_error": (C.c_char_p, []),
@@ -175,6 +202,7 @@ PROTOTYPES = {
     "hf_constants_set_sia_blake2b": (C.c_int, [C.c_void_p, C.c_char_p]),
     "hf_constants_set_blake2b": (C.c_int, [C.c_void_p, C.c_char_p]),
     "hf_plan_bind_constants": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "hf_workspace_bytes": (C.c_int, [C.c_char_p, C.c_void_p, C.POINTER(C.c_size_t)]),
     "hf_launch_native": (C.c_int, [C.c_char_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     "hf_launch_native_with": (C.c_int, [C.c_char_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     "hf_launch_fused": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),

@@ -83,6 +83,15 @@ bool lookup_kernel(const std::string &name, KernelId &id) {
   return false;
 }
 
+// Operators of token models: launched alone, by their own launches (launch.h).
+enum TokenOp { OP_LAYER_NORM, OP_LAYER_NORM_BACKWARD, OP_EMBEDDING, OP_EMBEDDING_BACKWARD, OP_NONE };
+TokenOp lookup_token_op(const std::string &name) {
+  static const char *const names[] = {"layer_norm_forward", "layer_norm_backward", "embedding_forward", "embedding_backward"};
+  for (int i = 0; i < OP_NONE; i++)
+    if (name == names[i]) return (TokenOp)i;
+  return OP_NONE;
+}
+
 // Barriers each built body executes (the YAML's HasBarriers is informational in the
 // reference as well: BarrierRewriter rewrites whatever __syncthreads it finds).
 bool body_has_barriers(KernelId id) { return id == K_BNSTATS || id == K_HISTC; }
@@ -494,6 +503,146 @@ int prepare_blake2b(const hf_blake2b_args &a, bool sia, const SearchConstants &c
 }
 
 // `consts`: the constants a search kernel is launched with; null = the process-wide set as it is now.
+// ------------------------------------------------ token-model operators
+bool element_type_ok(int t) { return t == HF_F32 || t == HF_BF16 || t == HF_F16; }
+size_t element_bytes(int t) { return t == HF_F32 ? 4 : 2; }
+bool aligned_to(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// One tensor of `rows` rows of `cols` elements; an output's rows must not overlap.  A tensor of no rows needs no pointer.
+int check_rows(const std::string &who, const char *name, const void *p, int64_t rows, int64_t cols, int64_t stride, int type,
+               bool output) {
+  int64_t reach;
+  if (rows == 0) return HF_OK;
+  if (!p) return fail(HF_EINVAL, who + "null " + name + " pointer");
+  if (!aligned_to(p, element_bytes(type))) return fail(HF_EINVAL, who + name + " is not aligned to its element type");
+  if (stride < 0 || !product(reach, {rows - 1, stride}) || reach + cols > kMaxOffset)
+    return fail(HF_EINVAL, who + "negative or oversized stride of " + name);
+  if (output && rows > 1 && stride < cols) return fail(HF_EINVAL, who + "the rows of " + name + " overlap");
+  return HF_OK;
+}
+
+int check_workspace(const std::string &who, size_t need, const void *p, size_t have) {
+  if (need == 0) return HF_OK;
+  if (!p || have < need)
+    return fail(HF_EINVAL, who + "needs " + std::to_string(need) + " bytes of workspace (hf_workspace_bytes), got " +
+                               std::to_string(p ? have : 0));
+  if (!aligned16(p)) return fail(HF_EINVAL, who + "workspace is not 16-byte aligned");
+  return HF_OK;
+}
+
+// Sizes and types only: what hf_workspace_bytes needs of an argument list.
+template <class A>
+int check_norm_sizes(const std::string &who, const A &a) {
+  if (!element_type_ok(a.type)) return fail(HF_EINVAL, who + "unknown element type");
+  if (a.param_type != a.type && a.param_type != HF_F32)
+    return fail(HF_EINVAL, who + "parameters must be of the rows' type or float32");
+  if (a.rows < 0 || !extent_ok(a.cols)) return fail(HF_EINVAL, who + "negative row count or no columns");
+  if (a.rows >= kMaxExtent) return fail(HF_EUNSUPPORTED, who + "2^31 rows or more are not built");
+  return HF_OK;
+}
+template <class A>
+int check_embedding_sizes(const std::string &who, const A &a) {
+  if (!element_type_ok(a.type)) return fail(HF_EINVAL, who + "unknown element type");
+  if (a.index_type != HF_I32 && a.index_type != HF_I64) return fail(HF_EINVAL, who + "unknown token type");
+  if (a.ntokens < 0 || !extent_ok(a.vocab) || !extent_ok(a.cols))
+    return fail(HF_EINVAL, who + "negative token count, no vocabulary or no columns");
+  if (a.ntokens >= kMaxExtent) return fail(HF_EUNSUPPORTED, who + "2^31 tokens or more are not built");
+  if (!std::isfinite(a.scale)) return fail(HF_EINVAL, who + "scale must be finite");
+  return HF_OK;
+}
+int check_params(const std::string &who, std::initializer_list<const void *> params, int type) {
+  for (const void *p : params)
+    if (p && !aligned_to(p, element_bytes(type))) return fail(HF_EINVAL, who + "a parameter is not aligned to its element type");
+  return HF_OK;
+}
+
+int check_layer_norm(const hf_layer_norm_args &a) {
+  const std::string who = "layer_norm_forward: ";
+  int rc = check_norm_sizes(who, a);
+  if (rc == HF_OK) rc = check_rows(who, "x", a.x, a.rows, a.cols, a.x_stride, a.type, false);
+  if (rc == HF_OK) rc = check_rows(who, "y", a.y, a.rows, a.cols, a.y_stride, a.type, true);
+  if (rc == HF_OK) rc = check_params(who, {a.weight, a.bias}, a.param_type);
+  if (rc == HF_OK) rc = check_params(who, {a.mean, a.rstd}, HF_F32);
+  if (rc == HF_OK && (!std::isfinite(a.eps) || a.eps < 0.0f)) rc = fail(HF_EINVAL, who + "eps must be finite and not negative");
+  return rc;
+}
+
+int check_layer_norm_backward(const hf_layer_norm_backward_args &a) {
+  const std::string who = "layer_norm_backward: ";
+  int rc = check_norm_sizes(who, a);
+  if (rc == HF_OK) rc = check_rows(who, "dy", a.dy, a.rows, a.cols, a.dy_stride, a.type, false);
+  if (rc == HF_OK && (a.dx || a.dweight)) {   // the bias's gradient alone is a sum of dy
+    rc = check_rows(who, "x", a.x, a.rows, a.cols, a.x_stride, a.type, false);
+    if (rc == HF_OK) rc = check_rows(who, "mean", a.mean, a.rows, 1, 1, HF_F32, false);
+    if (rc == HF_OK) rc = check_rows(who, "rstd", a.rstd, a.rows, 1, 1, HF_F32, false);
+  }
+  if (rc == HF_OK && a.dx) rc = check_rows(who, "dx", a.dx, a.rows, a.cols, a.dx_stride, a.type, true);
+  if (rc == HF_OK) rc = check_params(who, {a.weight, a.dweight, a.dbias}, a.param_type);
+  if (rc == HF_OK) rc = check_workspace(who, layer_norm_backward_workspace(a, cu_count()), a.workspace, a.workspace_bytes);
+  return rc;
+}
+
+int check_embedding(const hf_embedding_args &a) {
+  const std::string who = "embedding_forward: ";
+  int rc = check_embedding_sizes(who, a);
+  if (rc == HF_OK) rc = check_rows(who, "tokens", a.tokens, a.ntokens, 1, 1, HF_F32, false);
+  if (rc == HF_OK && a.index_type == HF_I64 && !aligned_to(a.tokens, 8)) rc = fail(HF_EINVAL, who + "tokens are not aligned to 8 bytes");
+  if (rc == HF_OK) rc = check_rows(who, "weight", a.weight, a.vocab, a.cols, a.weight_stride, a.type, false);
+  if (rc == HF_OK) rc = check_rows(who, "out", a.out, a.ntokens, a.cols, a.out_stride, a.type, true);
+  return rc;
+}
+
+int check_embedding_backward_sizes(const std::string &who, const hf_embedding_backward_args &a) {
+  int rc = check_embedding_sizes(who, a);
+  if (rc == HF_OK && a.out_type != a.type && a.out_type != HF_F32)
+    rc = fail(HF_EINVAL, who + "the gradient must be of dy's type or float32");
+  if (rc == HF_OK && a.padding_idx >= a.vocab) rc = fail(HF_EINVAL, who + "padding_idx is not in the vocabulary");
+  return rc;
+}
+
+int check_embedding_backward(const hf_embedding_backward_args &a) {
+  const std::string who = "embedding_backward: ";
+  int rc = check_embedding_backward_sizes(who, a);
+  if (rc == HF_OK) rc = check_rows(who, "tokens", a.tokens, a.ntokens, 1, 1, HF_F32, false);
+  if (rc == HF_OK && a.index_type == HF_I64 && !aligned_to(a.tokens, 8)) rc = fail(HF_EINVAL, who + "tokens are not aligned to 8 bytes");
+  if (rc == HF_OK) rc = check_rows(who, "dy", a.dy, a.ntokens, a.cols, a.dy_stride, a.type, false);
+  if (rc == HF_OK) rc = check_rows(who, "dweight", a.dweight, a.vocab, a.cols, a.dweight_stride, a.out_type, true);
+  if (rc == HF_OK) rc = check_workspace(who, embedding_backward_workspace(a, cu_count()), a.workspace, a.workspace_bytes);
+  return rc;
+}
+
+int launch_token_op(TokenOp op, const void *args, int grid_blocks, int block_threads, hipStream_t stream) {
+  if (!args) return fail(HF_EINVAL, "null argument list");
+  if (grid_blocks > 0 || block_threads > 0) return fail(HF_EINVAL, "this operator sizes its own launches: grid_blocks and block_threads must be <= 0");
+  int rc = HF_OK;
+  hipError_t e = hipSuccess;
+  switch (op) {
+    case OP_LAYER_NORM: {
+      const auto &a = *static_cast<const hf_layer_norm_args *>(args);
+      if ((rc = check_layer_norm(a)) == HF_OK) e = launch_layer_norm(a, cu_count(), stream);
+      break;
+    }
+    case OP_LAYER_NORM_BACKWARD: {
+      const auto &a = *static_cast<const hf_layer_norm_backward_args *>(args);
+      if ((rc = check_layer_norm_backward(a)) == HF_OK) e = launch_layer_norm_backward(a, cu_count(), stream);
+      break;
+    }
+    case OP_EMBEDDING: {
+      const auto &a = *static_cast<const hf_embedding_args *>(args);
+      if ((rc = check_embedding(a)) == HF_OK) e = launch_embedding(a, cu_count(), stream);
+      break;
+    }
+    case OP_EMBEDDING_BACKWARD: {
+      const auto &a = *static_cast<const hf_embedding_backward_args *>(args);
+      if ((rc = check_embedding_backward(a)) == HF_OK) e = launch_embedding_backward(a, cu_count(), stream);
+      break;
+    }
+    default: rc = fail(HF_ENOTFOUND, "unknown operator");
+  }
+  if (rc != HF_OK) return rc;
+  return e == hipSuccess ? HF_OK : hip_fail(e, "native launch");
+}
+
 int prepare(KernelId id, const void *args, Prepared &p, const SearchConstants *consts = nullptr) {
   if (!args) return fail(HF_EINVAL, "null argument list");
   p = Prepared();
@@ -772,6 +921,8 @@ HF_API int hf_plan_create(const hf_config *cfg, int fusion_index, const char *pr
   plan->n = (int)f.kernels.size();
   for (int i = 0; i < plan->n; i++) {
     plan->rows[i] = *cfg->cfg.find(f.kernels[i]);
+    if (lookup_token_op(plan->rows[i].name) != OP_NONE)
+      return fail(HF_EUNSUPPORTED, "'" + plan->rows[i].name + "' is launched alone (hf_launch_native): no fused kernel is built with it");
     if (!lookup_kernel(plan->rows[i].name, plan->ids[i]))
       return fail(HF_ENOTFOUND, "kernel '" + plan->rows[i].name + "' has no gfx950 implementation in this library");
   }
@@ -1206,6 +1357,8 @@ namespace {
 int launch_native_named(const char *kernel_name, const void *args, const SearchConstants *consts, int grid_blocks,
                         int block_threads, void *stream) {
   if (!kernel_name) return fail(HF_EINVAL, "null kernel name");
+  const TokenOp op = lookup_token_op(kernel_name);
+  if (op != OP_NONE) return launch_token_op(op, args, grid_blocks, block_threads, static_cast<hipStream_t>(stream));
   KernelId id;
   if (!lookup_kernel(kernel_name, id))
     return fail(HF_ENOTFOUND, std::string("kernel '") + kernel_name + "' has no gfx950 implementation in this library");
@@ -1221,6 +1374,35 @@ int launch_native_named(const char *kernel_name, const void *args, const SearchC
 HF_API int hf_launch_native(const char *kernel_name, const void *args, int grid_blocks, int block_threads,
                             void *stream) try {
   return launch_native_named(kernel_name, args, nullptr, grid_blocks, block_threads, stream);
+} catch (...) {
+  return trap_exception();
+}
+
+HF_API int hf_workspace_bytes(const char *kernel_name, const void *args, size_t *bytes) try {
+  if (!bytes) return fail(HF_EINVAL, "null output pointer");
+  *bytes = 0;
+  if (!kernel_name) return fail(HF_EINVAL, "null kernel name");
+  if (!args) return fail(HF_EINVAL, "null argument list");
+  int rc = HF_OK;
+  switch (lookup_token_op(kernel_name)) {
+    case OP_LAYER_NORM_BACKWARD: {
+      const auto &a = *static_cast<const hf_layer_norm_backward_args *>(args);
+      if ((rc = check_norm_sizes("layer_norm_backward: ", a)) == HF_OK) *bytes = layer_norm_backward_workspace(a, cu_count());
+      return rc;
+    }
+    case OP_EMBEDDING_BACKWARD: {
+      const auto &a = *static_cast<const hf_embedding_backward_args *>(args);
+      if ((rc = check_embedding_backward_sizes("embedding_backward: ", a)) == HF_OK) *bytes = embedding_backward_workspace(a, cu_count());
+      return rc;
+    }
+    case OP_LAYER_NORM:
+    case OP_EMBEDDING: return HF_OK;
+    default: break;
+  }
+  KernelId id;
+  if (!lookup_kernel(kernel_name, id))
+    return fail(HF_ENOTFOUND, std::string("kernel '") + kernel_name + "' has no gfx950 implementation in this library");
+  return HF_OK;
 } catch (...) {
   return trap_exception();
 }

@@ -4,6 +4,7 @@
 
 #include <cstddef>
 
+#include "../../include/hfuse_gfx950.h"
 #include "device/subblock.h"
 
 namespace hfuse {
@@ -40,5 +41,13 @@ hipError_t launch_copy_f32(const float *src, float *dst, unsigned long long n, h
 // The bare stream kernels (HF_STREAM_* patterns) over n4 16-byte vectors.
 hipError_t launch_stream_probe(int pattern, const void *src, void *dst, unsigned long long n4, unsigned grid, unsigned block,
                                hipStream_t stream);
+
+// Token-model operators.  `cus`: compute units of the device; the argument lists have been validated.
+size_t layer_norm_backward_workspace(const hf_layer_norm_backward_args &a, int cus);
+size_t embedding_backward_workspace(const hf_embedding_backward_args &a, int cus);
+hipError_t launch_layer_norm(const hf_layer_norm_args &a, int cus, hipStream_t stream);
+hipError_t launch_layer_norm_backward(const hf_layer_norm_backward_args &a, int cus, hipStream_t stream);
+hipError_t launch_embedding(const hf_embedding_args &a, int cus, hipStream_t stream);
+hipError_t launch_embedding_backward(const hf_embedding_backward_args &a, int cus, hipStream_t stream);
 
 }  // namespace hfuse

@@ -374,6 +374,70 @@ def histc_args(x, out, nbins, lo, hi) -> L.HistcArgs:
     return a
 
 
+# ------------------------------------------------------------ token-model operators
+def element_type(t) -> int:
+    """HF_F32 / HF_BF16 / HF_F16 of a tensor or dtype."""
+    import torch
+    return {torch.float32: L.HF_F32, torch.bfloat16: L.HF_BF16, torch.float16: L.HF_F16}[getattr(t, "dtype", t)]
+
+
+def index_type(t) -> int:
+    import torch
+    return {torch.int32: L.HF_I32, torch.int64: L.HF_I64}[t.dtype]
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _row_stride(t, cols: int) -> int:
+    """Elements between the rows of a [..., cols] tensor whose leading dimensions step evenly (any value for one row)."""
+    return t.stride(-2) if t.dim() == 2 and t.shape[0] > 1 else cols
+
+
+def layer_norm_args(x, y, weight=None, bias=None, mean=None, rstd=None, eps: float = 1e-5) -> L.LayerNormArgs:
+    """x, y: [rows, cols], their rows dense; weight / bias: [cols]; mean / rstd: [rows] float32."""
+    rows, cols = x.shape
+    param = weight if weight is not None else bias
+    return L.LayerNormArgs(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean), _ptr(rstd), rows, cols,
+                           _row_stride(x, cols), _row_stride(y, cols), eps, element_type(x),
+                           element_type(x if param is None else param))
+
+
+def layer_norm_backward_args(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=None,
+                             workspace=None) -> L.LayerNormBackwardArgs:
+    """dy, x, dx: [rows, cols]; dweight / dbias: [cols] of the parameters' type; workspace: a byte tensor of workspace_bytes()."""
+    rows, cols = x.shape
+    param = next((t for t in (weight, dweight, dbias) if t is not None), x)
+    return L.LayerNormBackwardArgs(_ptr(dy), _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight), _ptr(dbias),
+                                   rows, cols, _row_stride(dy, cols), _row_stride(x, cols),
+                                   cols if dx is None else _row_stride(dx, cols), element_type(x), element_type(param),
+                                   _ptr(workspace), 0 if workspace is None else workspace.numel())
+
+
+def embedding_args(tokens, weight, out, scale: float = 1.0) -> L.EmbeddingArgs:
+    """tokens: int32 / int64, contiguous; weight: [vocab, cols]; out: [tokens, cols]."""
+    vocab, cols = weight.shape
+    return L.EmbeddingArgs(_ptr(tokens), _ptr(weight), _ptr(out), tokens.numel(), vocab, cols, _row_stride(weight, cols),
+                           _row_stride(out, cols), scale, element_type(weight), index_type(tokens))
+
+
+def embedding_backward_args(dy, tokens, dweight, scale: float = 1.0, padding_idx: int = -1,
+                            workspace=None) -> L.EmbeddingBackwardArgs:
+    """dy: [tokens, cols]; dweight: [vocab, cols]; padding_idx < 0: none; workspace: a byte tensor of workspace_bytes()."""
+    vocab, cols = dweight.shape
+    return L.EmbeddingBackwardArgs(_ptr(dy), _ptr(tokens), _ptr(dweight), tokens.numel(), vocab, cols, _row_stride(dy, cols),
+                                   _row_stride(dweight, cols), padding_idx, scale, element_type(dy), element_type(dweight),
+                                   index_type(tokens), _ptr(workspace), 0 if workspace is None else workspace.numel())
+
+
+def workspace_bytes(kernel_name: str, args) -> int:
+    """Device bytes a native launch of this argument list needs as its workspace."""
+    n = C.c_size_t()
+    check(L.lib().hf_workspace_bytes(kernel_name.encode(), C.byref(args), C.byref(n)))
+    return n.value
+
+
 # ------------------------------------------------------------ searches
 def new_search_results(device="cuda"):
     """Zeroed device buffer holding one hf_search_results."""

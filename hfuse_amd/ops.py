@@ -17,9 +17,19 @@ and `ethash_search` upload a job's constants and return an op; `hits(op)` reads 
 Tensors are float32 CUDA tensors (this build's kernels are the float instantiations the
 reference fused); inputs are made contiguous where the original operator does so.  torch is used
 for allocation and streams only; every launch goes through the C-ABI.
+
+The operators of token models (`embedding`, `layer_norm` and their gradients) take float32, bfloat16 and
+float16, and are launched alone:
+
+    (h,) = ops.run(ops.embedding(tokens, table, scale))
+    y, mean, rstd = ops.run(ops.layer_norm(h, h.shape[-1], weight, bias))
+    dh, dweight, dbias = ops.run(ops.layer_norm_backward(dy, h, h.shape[-1], mean, rstd, weight))
+    (dtable,) = ops.run(ops.embedding_backward(dh, tokens, table.shape[0], scale))
 """
 from __future__ import annotations
 
+import math
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Any, Optional, Sequence, Tuple
 
@@ -47,6 +57,7 @@ class Op:
     args: Any
     outputs: Tuple[Any, ...]
     keep: Tuple[Any, ...] = ()
+    device: Any = None     # token-model operators: where their tensors live
 
 
 def im2col(x, kernel_size, dilation=1, padding=0, stride=1) -> Op:
@@ -136,6 +147,185 @@ def histc(x, bins: int = 100, min: float = 0.0, max: float = 0.0) -> Op:
     return Op("kernelHistogram1D", H.histc_args(flat, out, int(bins), lo, hi), (out,), (flat, out))
 
 
+# ------------------------------------------------------------------ token-model operators
+_DTYPES = ("float32", "bfloat16", "float16")
+
+
+def _check_typed(x, what: str, name: str):
+    import torch
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: {name} must be a CUDA tensor of {', '.join(_DTYPES)}")
+
+
+def _check_same_device(what: str, x, *others):
+    for t in others:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
+
+
+def _as_rows(x, rows: int, cols: int):
+    """x as [rows, cols] with dense rows: a view where its strides allow it, else a contiguous copy."""
+    if x.is_contiguous():
+        return x.view(rows, cols)
+    try:
+        v = x.view(rows, cols)
+    except RuntimeError:
+        return x.contiguous().view(rows, cols)
+    return v if cols == 1 or v.stride(1) == 1 else v.contiguous()
+
+
+def _workspace(kernel: str, args, device):
+    import torch
+    need = H.workspace_bytes(kernel, args)
+    if not need:
+        return None
+    ws = torch.empty(need, device=device, dtype=torch.uint8)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    return ws
+
+
+def _check_tokens(tokens, what: str):
+    import torch
+    if not isinstance(tokens, torch.Tensor) or not tokens.is_cuda or tokens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: tokens must be an int32 or int64 CUDA tensor")
+    return tokens.contiguous()
+
+
+def _check_scale(scale, what: str) -> float:
+    scale = float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"{what}: scale must be finite")
+    return scale
+
+
+def embedding(tokens, weight, scale: float = 1.0) -> Op:
+    """scale * weight[tokens]: tokens [...] int32 / int64, weight [V, D] -> [..., D] of weight's type.
+
+    A token outside [0, V), such as the -1 behind the last token of a padded sequence, looks up a row of zeros."""
+    import torch
+    _check_typed(weight, "embedding", "weight")
+    tok = _check_tokens(tokens, "embedding")
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise ValueError("embedding: weight must be a non-empty [vocabulary, columns] tensor")
+    scale = _check_scale(scale, "embedding")
+    _check_same_device("embedding", weight, tok)
+    vocab, cols = weight.shape
+    w = _as_rows(weight, vocab, cols)
+    out = torch.empty((tok.numel(), cols), device=weight.device, dtype=weight.dtype)
+    return Op("embedding_forward", H.embedding_args(tok, w, out, scale), (out.view(tokens.shape + (cols,)),), (tok, w, out),
+              weight.device)
+
+
+def embedding_backward(dy, tokens, num_embeddings: int, scale: float = 1.0, padding_idx: Optional[int] = None,
+                       dtype=None) -> Op:
+    """Gradient of `embedding` with respect to its weight: dy [..., D] -> [num_embeddings, D] of dy's type or float32 (`dtype`).
+
+    Row v is scale times the sum of the dy rows whose token is v, summed in 32 bits in the order of the tokens; the row of
+    `padding_idx` is zeros, and the dy rows of that token and of tokens outside [0, num_embeddings) are not read."""
+    import torch
+    what = "embedding_backward"
+    _check_typed(dy, what, "dy")
+    tok = _check_tokens(tokens, what)
+    scale = _check_scale(scale, what)
+    vocab = int(num_embeddings)
+    if vocab <= 0:
+        raise ValueError(f"{what}: num_embeddings must be positive")
+    if dy.dim() == 0 or dy.shape[:-1] != tokens.shape or dy.shape[-1] == 0:
+        raise ValueError(f"{what}: dy must be the tokens' shape {tuple(tokens.shape)} and the columns, got {tuple(dy.shape)}")
+    if padding_idx is not None and not 0 <= int(padding_idx) < vocab:
+        raise ValueError(f"{what}: padding_idx is not in the vocabulary")
+    dtype = dy.dtype if dtype is None else dtype
+    if dtype not in (dy.dtype, torch.float32):
+        raise TypeError(f"{what}: the gradient is of dy's type or float32")
+    _check_same_device(what, dy, tok)
+    cols = dy.shape[-1]
+    g = _as_rows(dy, tok.numel(), cols)
+    out = torch.empty((vocab, cols), device=dy.device, dtype=dtype)
+    args = H.embedding_backward_args(g, tok, out, scale, -1 if padding_idx is None else int(padding_idx))
+    return Op("embedding_backward", args, (out,), (tok, g, out, _workspace("embedding_backward", args, dy.device)), dy.device)
+
+
+def _norm_shape(x, normalized_shape, what: str) -> Tuple[int, ...]:
+    shape = (int(normalized_shape),) if isinstance(normalized_shape, int) else tuple(int(n) for n in normalized_shape)
+    if not shape or x.dim() < len(shape) or tuple(x.shape[-len(shape):]) != shape or math.prod(shape) == 0:
+        raise ValueError(f"{what}: normalized_shape {shape} is not the (non-empty) end of the input's shape {tuple(x.shape)}")
+    return shape
+
+
+def _norm_param(p, x, shape, what: str, name: str):
+    import torch
+    if p is None:
+        return None
+    _check_typed(p, what, name)
+    if tuple(p.shape) != shape:
+        raise ValueError(f"{what}: {name} must have the shape {shape}, got {tuple(p.shape)}")
+    if p.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"{what}: {name} must be of the input's type or float32")
+    return p.contiguous()
+
+
+def layer_norm(x, normalized_shape, weight=None, bias=None, eps: float = 1e-5) -> Op:
+    """torch.native_layer_norm: x [..., *normalized_shape] -> (y, mean, rstd), mean and rstd float32 [..., 1, ...].
+
+    weight and bias are both of x's type or both float32; y is of x's type."""
+    import torch
+    what = "layer_norm"
+    _check_typed(x, what, "x")
+    shape = _norm_shape(x, normalized_shape, what)
+    w, b = _norm_param(weight, x, shape, what, "weight"), _norm_param(bias, x, shape, what, "bias")
+    if w is not None and b is not None and w.dtype != b.dtype:
+        raise TypeError(f"{what}: weight and bias must be of one type")
+    eps = float(eps)
+    if not (math.isfinite(eps) and eps >= 0.0):
+        raise ValueError(f"{what}: eps must be finite and not negative")
+    _check_same_device(what, x, w, b)
+    cols = math.prod(shape)
+    rows = x.numel() // cols
+    x2 = _as_rows(x, rows, cols)
+    y = torch.empty((rows, cols), device=x.device, dtype=x.dtype)
+    mean = torch.empty(rows, device=x.device, dtype=torch.float32)
+    rstd = torch.empty(rows, device=x.device, dtype=torch.float32)
+    stat = tuple(x.shape[:x.dim() - len(shape)]) + (1,) * len(shape)
+    return Op("layer_norm_forward", H.layer_norm_args(x2, y, w, b, mean, rstd, eps),
+              (y.view(x.shape), mean.view(stat), rstd.view(stat)), (x2, w, b, y, mean, rstd), x.device)
+
+
+def layer_norm_backward(dy, x, normalized_shape, mean, rstd, weight=None,
+                        output_mask: Optional[Sequence[bool]] = None) -> Op:
+    """torch.native_layer_norm_backward: -> (dx, dweight, dbias) with the mean and rstd that `layer_norm` gave for x.
+
+    `output_mask` says which of the three are wanted, the others come back as None (default: dx, and the parameters'
+    gradients where there is a weight).  dweight and dbias are of weight's type (x's without one)."""
+    import torch
+    what = "layer_norm_backward"
+    _check_typed(x, what, "x")
+    _check_typed(dy, what, "dy")
+    shape = _norm_shape(x, normalized_shape, what)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"{what}: dy must have x's shape and type")
+    w = _norm_param(weight, x, shape, what, "weight")
+    cols = math.prod(shape)
+    rows = x.numel() // cols
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32:
+            raise TypeError(f"{what}: {name} must be a float32 CUDA tensor")
+        if t.numel() != rows:
+            raise ValueError(f"{what}: {name} must hold one value a row")
+    mask = (True, w is not None, w is not None) if output_mask is None else tuple(bool(m) for m in output_mask)
+    if len(mask) != 3 or not any(mask):
+        raise ValueError(f"{what}: output_mask must be three flags, one of them set")
+    _check_same_device(what, x, dy, mean, rstd, w)
+    dy2, x2, mean, rstd = _as_rows(dy, rows, cols), _as_rows(x, rows, cols), mean.contiguous(), rstd.contiguous()
+    ptype = x.dtype if w is None else w.dtype
+    dx = torch.empty((rows, cols), device=x.device, dtype=x.dtype) if mask[0] else None
+    dw = torch.empty(cols, device=x.device, dtype=ptype) if mask[1] else None
+    db = torch.empty(cols, device=x.device, dtype=ptype) if mask[2] else None
+    args = H.layer_norm_backward_args(dy2, x2, mean, rstd, w, dx, dw, db)
+    return Op("layer_norm_backward", args,
+              (dx if dx is None else dx.view(x.shape), dw if dw is None else dw.view(shape), db if db is None else db.view(shape)),
+              (dy2, x2, mean, rstd, w, dx, dw, db, _workspace("layer_norm_backward", args, x.device)), x.device)
+
+
 # ------------------------------------------------------------------ nonce searches
 # The miners' host loop: constants of a search (header, target, DAG) are uploaded once per
 # job, then a launch scans `count` nonces from `start` and appends its hits to a result record.
@@ -199,12 +389,31 @@ def _config(cfg: Optional[H.Config]) -> H.Config:
 
 
 def run(op: Op, stream=None):
-    """Launch one original kernel; returns its outputs (a tuple)."""
+    """Launch one original kernel; returns its outputs (a tuple).
+
+    A token-model operator runs on its tensors' device, and its tensors are recorded on `stream` where that is not the
+    current stream, so that they may be dropped as soon as the call returns."""
+    if op.device is not None:
+        return _run_on_device(op, stream)
     count = getattr(op, "count", 0)
     if count:   # ethash: grid * 128 threads cover the requested nonces
         H.launch_native(op.kernel, op.args, (count + 127) // 128, 128, stream=stream)
     else:
         H.launch_native(op.kernel, op.args, stream=stream)
+    return op.outputs
+
+
+def _run_on_device(op: Op, stream):
+    import torch
+    index = op.device.index
+    with nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index):
+        H.launch_native(op.kernel, op.args, stream=stream)
+        if stream is not None:
+            used = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream), device=op.device)
+            if used != torch.cuda.current_stream():
+                for t in op.keep:
+                    if t is not None:
+                        t.record_stream(used)
     return op.outputs
 
 

@@ -425,6 +425,86 @@ typedef struct {
   uint32_t target2[2]; /* uint2: {low, high} words of the 64-bit target */
 } hf_blake2b_args;
 
+/* ------------------------------------------------- token-model operators */
+/*
+ * Layer norm and token embedding with their gradients (no counterpart in the reference, whose kernels are those of
+ * image models): "layer_norm_forward", "layer_norm_backward", "embedding_forward", "embedding_backward" for
+ * hf_launch_native.  They choose their own launches, of one kernel or of several in order on the stream, so
+ * grid_blocks and block_threads must be <= 0, and they are launched alone: a fusion list that names one loads, and
+ * hf_plan_create answers HF_EUNSUPPORTED.
+ *
+ * Rows are `cols` adjacent elements; row i of a tensor starts at element i * stride, a stride >= 0 of any alignment (0
+ * for an input repeats one row).  Outputs must not overlap inputs or each other.  Sums, means and variances are held in
+ * 32 bits, and every output is rounded once, to nearest even.  No result depends on the order in which workgroups
+ * finish: the same call gives the same bits.  Zero rows or tokens are legal (the gradients of parameters are then zeros).
+ */
+enum { HF_F32 = 0, HF_BF16 = 1, HF_F16 = 2 };   /* element types  */
+enum { HF_I32 = 0, HF_I64 = 1 };                /* token id types */
+
+/*
+ * y = (x - mean(x)) / sqrt(var(x) + eps) * weight + bias for each row, var the mean square of x - mean(x).
+ * weight / bias: `cols` elements of param_type (the rows' type or HF_F32), each may be NULL (ones / zeros).
+ * mean / rstd: the statistics of every row, each may be NULL.
+ */
+typedef struct {
+  const void *x, *weight, *bias;
+  void *y;
+  float *mean, *rstd;
+  int64_t rows, cols, x_stride, y_stride;
+  float eps;
+  int type, param_type;
+} hf_layer_norm_args;
+
+/*
+ * With h = (x - mean) * rstd and g = dy * weight: dx = rstd * (g - mean(g) - h * mean(g * h)) for each row,
+ * dweight = sum over the rows of dy * h, dbias = sum over the rows of dy.  dx, dweight and dbias may each be NULL (not
+ * wanted).  dweight and dbias are of param_type.  workspace: hf_workspace_bytes of this argument list, 16-byte aligned;
+ * its contents mean nothing before or after, and two calls that may run at the same time need one each.
+ */
+typedef struct {
+  const void *dy, *x, *weight;
+  const float *mean, *rstd;
+  void *dx, *dweight, *dbias;
+  int64_t rows, cols, dy_stride, x_stride, dx_stride;
+  int type, param_type;
+  void *workspace;
+  size_t workspace_bytes;
+} hf_layer_norm_backward_args;
+
+/*
+ * out row i = scale * weight row tokens[i], one rounding (scale 1 copies the bits of every number); a row of zeros where
+ * tokens[i] is outside [0, vocab), such as the -1 behind the last token of a padded sequence.
+ */
+typedef struct {
+  const void *tokens, *weight;
+  void *out;
+  int64_t ntokens, vocab, cols, weight_stride, out_stride;
+  float scale;
+  int type, index_type;
+} hf_embedding_args;
+
+/*
+ * dweight row v = scale * (sum of the dy rows i with tokens[i] == v), in the order of i; zeros where no token names v and
+ * for v == padding_idx (< 0: none).  All `vocab` rows are written.  The dy rows of tokens outside [0, vocab) or equal to
+ * padding_idx are not read.  out_type is the type of dy or HF_F32.  workspace as for hf_layer_norm_backward_args.
+ */
+typedef struct {
+  const void *dy, *tokens;
+  void *dweight;
+  int64_t ntokens, vocab, cols, dy_stride, dweight_stride, padding_idx;
+  float scale;
+  int type, out_type, index_type;
+  void *workspace;
+  size_t workspace_bytes;
+} hf_embedding_backward_args;
+
+/*
+ * *bytes = the device memory that a native launch of this argument list needs as its `workspace` on the current device
+ * (0 for kernels without one).  The sizes, types and wanted outputs are read; data and workspace pointers may be NULL,
+ * except that an output left NULL counts as not wanted.
+ */
+HF_API int hf_workspace_bytes(const char *kernel_name, const void *args, size_t *bytes);
+
 /*
  * Constants the original kernels read from __constant__ symbols set by their
  * host program (DAG pointer and size, header, midstate, target).  The library

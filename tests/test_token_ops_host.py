@@ -1,0 +1,120 @@
+"""Token-model operators: what they refuse, on the CPU, before anything is launched (pointers here are never read)."""
+import ctypes as C
+
+import pytest
+import torch
+
+import hfuse_amd
+from hfuse_amd import _lib as L
+from hfuse_amd import launcher as H
+from hfuse_amd import ops
+from hfuse_amd.launcher import Config
+
+P = 1 << 20        # a well-aligned address
+
+
+def norm(**kw):
+    a = L.LayerNormArgs(x=P, weight=P, bias=P, y=2 * P, mean=3 * P, rstd=3 * P, rows=4, cols=64, x_stride=64, y_stride=64, eps=1e-5)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def norm_grad(**kw):
+    a = L.LayerNormBackwardArgs(dy=P, x=P, weight=P, mean=P, rstd=P, dx=2 * P, dweight=3 * P, dbias=4 * P, rows=4, cols=64,
+                                dy_stride=64, x_stride=64, dx_stride=64, workspace=8 * P, workspace_bytes=1 << 40)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def lookup(**kw):
+    a = L.EmbeddingArgs(tokens=P, weight=P, out=2 * P, ntokens=4, vocab=10, cols=64, weight_stride=64, out_stride=64, scale=1.0,
+                        index_type=L.HF_I64)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def lookup_grad(**kw):
+    a = L.EmbeddingBackwardArgs(dy=P, tokens=P, dweight=2 * P, ntokens=4, vocab=10, cols=64, dy_stride=64, dweight_stride=64,
+                                padding_idx=-1, scale=1.0, index_type=L.HF_I64, workspace=8 * P, workspace_bytes=1 << 40)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+BAD = [
+    ("layer_norm_forward", norm, [dict(x=None), dict(y=None), dict(x=P + 2), dict(y=P + 1), dict(weight=P + 2), dict(mean=P + 1),
+                                  dict(rows=-1), dict(rows=1 << 31), dict(cols=0), dict(cols=1 << 31), dict(x_stride=-64),
+                                  dict(y_stride=63), dict(x_stride=1 << 62), dict(eps=-1.0), dict(eps=float("nan")),
+                                  dict(eps=float("inf")), dict(type=3), dict(type=-1), dict(type=L.HF_F32, param_type=L.HF_F16),
+                                  dict(type=L.HF_BF16, param_type=L.HF_F16)]),
+    ("layer_norm_backward", norm_grad, [dict(dy=None), dict(x=None), dict(mean=None), dict(rstd=None), dict(dx=P + 2), dict(dx_stride=10),
+                                        dict(dy_stride=-1), dict(rows=-1), dict(cols=-5), dict(type=7), dict(param_type=L.HF_BF16),
+                                        dict(dweight=P + 1), dict(dbias=P + 2)]),
+    ("embedding_forward", lookup, [dict(tokens=None), dict(tokens=P + 4), dict(weight=None), dict(out=None), dict(out_stride=1),
+                                   dict(weight_stride=-1), dict(ntokens=-1), dict(ntokens=1 << 31), dict(vocab=0), dict(cols=0),
+                                   dict(scale=float("inf")), dict(scale=float("nan")), dict(type=4), dict(index_type=2)]),
+    ("embedding_backward", lookup_grad, [dict(dy=None), dict(tokens=None), dict(dweight=None), dict(dweight_stride=63), dict(dy_stride=-2),
+                                         dict(padding_idx=10), dict(ntokens=-1), dict(vocab=-1), dict(vocab=1 << 31), dict(cols=0),
+                                         dict(scale=float("nan")), dict(type=L.HF_F32, out_type=L.HF_F16),
+                                         dict(type=L.HF_BF16, out_type=L.HF_F16), dict(index_type=-1), dict(tokens=P + 2)]),
+]
+
+
+@pytest.mark.parametrize("name, make, change", [(n, m, c) for n, m, cs in BAD for c in cs], ids=lambda v: str(v) if isinstance(v, dict) else "")
+def test_argument_lists_are_refused(name, make, change):
+    with pytest.raises(hfuse_amd.HfuseError) as e:
+        H.launch_native(name, make(**change), stream=0)
+    assert e.value.code in (L.HF_EINVAL, L.HF_EUNSUPPORTED) and name in e.value.message
+
+
+@pytest.mark.parametrize("name, make, _", BAD, ids=lambda v: v if isinstance(v, str) else "")
+def test_launch_shapes_and_null_lists_are_refused(name, make, _):
+    for kw in (dict(grid_blocks=4), dict(block_threads=256)):
+        with pytest.raises(hfuse_amd.HfuseError) as e:
+            H.launch_native(name, make(), stream=0, **kw)
+        assert e.value.code == L.HF_EINVAL and "sizes its own launches" in e.value.message
+    assert L.lib().hf_launch_native(name.encode(), None, 0, 0, None) == L.HF_EINVAL
+    assert L.lib().hf_workspace_bytes(name.encode(), None, C.byref(C.c_size_t())) == L.HF_EINVAL
+
+
+def test_workspace_sizes():
+    lib = L.lib()
+    n = C.c_size_t(7)
+    assert lib.hf_workspace_bytes(b"im2col_kernel", C.byref(L.Im2colArgs()), C.byref(n)) == 0 and n.value == 0
+    assert lib.hf_workspace_bytes(b"no_such_kernel", C.byref(norm()), C.byref(n)) == L.HF_ENOTFOUND
+    assert lib.hf_workspace_bytes(b"embedding_forward", C.byref(lookup()), None) == L.HF_EINVAL
+    assert H.workspace_bytes("layer_norm_forward", norm()) == 0 and H.workspace_bytes("embedding_forward", lookup()) == 0
+    for name, make in (("layer_norm_backward", norm_grad), ("embedding_backward", lookup_grad)):
+        need = H.workspace_bytes(name, make(workspace=None, workspace_bytes=0))
+        if need:    # too little, none at all, or off its alignment
+            for change in (dict(workspace_bytes=need - 1), dict(workspace=None), dict(workspace=8 * P + 8)):
+                with pytest.raises(hfuse_amd.HfuseError) as e:
+                    H.launch_native(name, make(**change), stream=0)
+                assert e.value.code == L.HF_EINVAL and "workspace" in e.value.message
+        with pytest.raises(hfuse_amd.HfuseError):
+            H.workspace_bytes(name, make(cols=-1))
+
+
+def test_nothing_to_do_needs_no_pointers():
+    H.launch_native("layer_norm_forward", norm(rows=0, x=None, y=None), stream=0)
+    H.launch_native("embedding_forward", lookup(ntokens=0, tokens=None, out=None), stream=0)
+
+
+def test_fusion_lists_cannot_name_them():
+    table = "".join(f"{k}:\n  KernelName: {k}\n  HasBarriers: false\n  BlockDim:\n    X: 256\n    Y: 1\n    Z: 1\n  Reg: 32\n"
+                    for k in ("layer_norm_forward", "MaxPoolForward"))
+    cfg = Config("- File: f\n  Kernels:\n    - layer_norm_forward\n    - MaxPoolForward\n", table)
+    with pytest.raises(hfuse_amd.HfuseError) as e:
+        cfg.plan(0, "hfuse")
+    assert e.value.code == L.HF_EUNSUPPORTED and "alone" in e.value.message
+
+
+def test_operators_refuse_cpu_tensors():
+    x, t = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)
+    for make in (lambda: ops.layer_norm(x, 8), lambda: ops.layer_norm_backward(x, x, 8, x[:, 0], x[:, 0]), lambda: ops.embedding(t, x),
+                 lambda: ops.embedding_backward(x, t, 10)):
+        with pytest.raises(TypeError):
+            make()
