@@ -19,8 +19,81 @@ __device__ __forceinline__ T from_f32(float v) {
   return (T)v;   // round to nearest even (v_cvt_pk_bf16_f32 / v_cvt_f16_f32)
 }
 
+// N adjacent elements.  Rows may start at any element, so the types used for memory are aligned to one element only
+// (gfx950 loads 16 bytes from any address; a wave's 1 KiB then touches nine 128-byte lines instead of eight).
+template <class T, int N>
+struct VecOf {
+  typedef T type __attribute__((ext_vector_type(N)));
+  typedef type mem __attribute__((aligned(sizeof(T))));
+};
+template <class T>
+struct VecOf<T, 1> {
+  typedef T type;
+  typedef T mem;
+};
+template <class T, int N>
+using vec_t = typename VecOf<T, N>::type;
+
+// Elements of a 16-byte access, the width of every row access where a row is that long.
+template <class T>
+constexpr int kVec = 16 / (int)sizeof(T);
+
+template <class T, int N>
+__device__ __forceinline__ vec_t<T, N> load_vec(const T *p) {
+  return *reinterpret_cast<const typename VecOf<T, N>::mem *>(p);
+}
+template <class T, int N>
+__device__ __forceinline__ vec_t<T, N> load_vec_stream(const T *p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const typename VecOf<T, N>::mem *>(p));
+}
+template <class T, int N>
+__device__ __forceinline__ void store_vec(T *p, vec_t<T, N> v) {
+  *reinterpret_cast<typename VecOf<T, N>::mem *>(p) = v;
+}
+template <class T, int N>
+__device__ __forceinline__ void store_vec_stream(T *p, vec_t<T, N> v) {
+  __builtin_nontemporal_store(v, reinterpret_cast<typename VecOf<T, N>::mem *>(p));
+}
+template <class T, int N>
+__device__ __forceinline__ float elem(const vec_t<T, N> &v, int i) {
+  if constexpr (N == 1) return to_f32(v);
+  else return to_f32(v[i]);
+}
+template <class T, int N>
+__device__ __forceinline__ vec_t<T, N> round_vec(const float *f) {
+  vec_t<T, N> v;
+  if constexpr (N == 1) v = from_f32<T>(f[0]);
+  else {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = from_f32<T>(f[i]);
+  }
+  return v;
+}
+
+// A row of `cols` elements (cols >= N) is covered by ceil(cols / N) accesses of N elements.  Where N does not divide cols
+// the last one is moved back to end with the row: it repeats elements of the one before, and stores to them repeat the
+// same values.  Slot j starts at column slot_column(j); its first slot_repeats(j) elements are repeats.
+template <int N>
+__device__ __forceinline__ int row_slots(int cols) {
+  return (int)(((unsigned)cols + (N - 1)) / N);
+}
+template <int N>
+__device__ __forceinline__ int slot_column(int j, int cols) {
+  return min(j * N, cols - N);
+}
+template <int N>
+__device__ __forceinline__ int slot_repeats(int j, int cols) {
+  return max(0, j * N - (cols - N));
+}
+
 // Sum over the 64 lanes, in every lane: a butterfly, so the order of the additions is fixed.
 __device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+__device__ __forceinline__ unsigned wave_sum_u32(unsigned v) {
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
   return v;
