@@ -23,272 +23,320 @@ __global__ __launch_bounds__(kThreads) void embedding_kernel(hf_embedding_args a
 }
 
 // ------------------------------------------------------------------ the gradient of the table
-// Three launches.  (1) group_tokens_kernel sorts the positions by token, stably, and writes the rows of zeros.
-// (2) sum_rows_kernel sums the dy rows of each token.  (3) join_rows_kernel adds up the tokens whose rows were shared out.
+// The usable tokens are sorted with their positions by a stable radix sort (count_digits_kernel and place_digits_kernel
+// for each digit), the dy rows of each token are summed from the sorted list (sum_rows_kernel), and tokens whose rows were
+// shared out are joined (join_rows_kernel).  The rows of zeros -- most of the table in a small batch -- are written by
+// further workgroups of the sort's launches: a sort of some thousand tokens waits for memory most of the time on a few
+// CUs and leaves the rest of the part and its write bandwidth to them.
 // No floating-point atomics: every sum has one order, whatever the order in which workgroups run.
+
+constexpr int kSortWaves = 4;
+constexpr int kSortThreads = 64 * kSortWaves;
+constexpr int kSortKeys = 4;                              // tokens a thread has in one step
+constexpr int kSortStep = kSortThreads * kSortKeys;
+constexpr int kMaxDigitBits = 9;
+constexpr int kMaxBuckets = 1 << kMaxDigitBits;
+constexpr int kSortTiles = 128;                           // workgroups of a sort launch at most
 
 // What the launches hand on, in the caller's workspace.
 struct TableScratch {
-  uint2 *order;        // {position, token} sorted by token, positions ascending
-  unsigned *starts;    // starts[v]: first entry of token v in `order`; starts[vocab] = number of usable tokens
-  unsigned *nlong;     // tokens whose rows more than one chunk sums ...
-  unsigned *longs;     // ... each by the chunk it starts in
-  float *partial;      // two rows of sums a chunk: of the token it starts inside of, and of the token it ends inside of
-  int chunk;           // entries a chunk has
-  int nchunks;
+  uint2 *order, *other;     // {position, token} sorted by token, positions ascending; the list before the last digit
+  unsigned *counts;         // [tile][bucket] of the digit in hand
+  unsigned *owner;          // owner[v] = a position that names token v, if any does; anything otherwise
+  unsigned *last;           // per shared token: the last chunk with a row of it
+  unsigned *state;          // [0] usable tokens, [1] shared tokens
+  unsigned *shared;         // the shared tokens, each by the chunk it starts in
+  float *partial;           // two rows of sums a chunk: of the token it begins inside of, and of the token it ends inside of
+  unsigned tile, tiles;     // positions of a sort workgroup (a multiple of kSortStep), sort workgroups
+  unsigned chunk, nchunks;  // entries summed by one group of lanes
 };
 
-constexpr int kGroupThreads = 1024;
-constexpr int kGroupWaves = kGroupThreads / 64;
-constexpr int kMaxRange = 768;             // tokens of a workgroup's range: a thread each, and 48 KiB of counters
-constexpr int kHitWords = 64;              // 64-bit words a wave has to remember which of its loads held a token of the range
+// Rows [row, row + rows) of the gradient, 2^lanes_log2 lanes each: those that no token names become zeros.
+struct ZeroRows {
+  unsigned row, rows;
+  int lanes_log2;
+  unsigned element;   // bytes of an element
+};
 
-// A usable token, or ~0 for one outside the table or equal to padding_idx.
 template <class I>
-__device__ __forceinline__ unsigned token_key(const I *tokens, unsigned i, unsigned n, unsigned vocab, unsigned pad) {
-  if (i >= n) return ~0u;
-  unsigned lo, hi = 0;
-  if constexpr (sizeof(I) == 8) {
-    const uint2 t = reinterpret_cast<const uint2 *>(tokens)[i];
-    lo = t.x;
-    hi = t.y;
+__device__ __forceinline__ void write_zero_rows(const hf_embedding_backward_args &a, const unsigned *owner, const ZeroRows &z, unsigned block) {
+  const size_t at = (size_t)block * 256u + threadIdx.x;
+  const size_t r = at >> z.lanes_log2;
+  if (r >= z.rows) return;
+  const size_t v = z.row + r;
+  // `owner` was never cleared: what it says is a claim, true if the position it gives names this token
+  const unsigned i = owner[v];
+  if (i < (unsigned)a.ntokens && (int64_t) static_cast<const I *>(a.tokens)[i] == (int64_t)v && (int64_t)v != a.padding_idx) return;
+  const unsigned lanes = 1u << z.lanes_log2, lane = (unsigned)at & (lanes - 1);
+  const unsigned bytes = (unsigned)a.cols * z.element;
+  unsigned char *row = static_cast<unsigned char *>(a.dweight) + v * (size_t)a.dweight_stride * z.element;
+  typedef unsigned short word_t;   // rows are aligned to an element, of two bytes or more
+  if (bytes >= 16) {
+    for (unsigned j = lane * 16u; j < bytes; j += lanes * 16u)
+      store_vec_stream<word_t, 8>(reinterpret_cast<word_t *>(row + min(j, bytes - 16u)), (vec_t<word_t, 8>)(word_t)0);
   } else {
-    lo = (unsigned)tokens[i];
+    for (unsigned j = lane * 2u; j < bytes; j += lanes * 2u) *reinterpret_cast<word_t *>(row + j) = 0;
   }
-  return (hi == 0 && lo < vocab && lo != pad) ? lo : ~0u;
 }
 
-// Each workgroup owns the tokens [first, first + range) and looks through all positions twice: it counts, lays its tokens
-// out behind those of the ranges below (which it counted as well), and places their positions.  A wave takes one
-// contiguous part of the positions and has counters of its own, so that positions come out in order.  Between the two
-// looks it writes zeros to the rows of its tokens that no position names, whose stores drain under the second look.
-template <class I>
-__global__ __launch_bounds__(kGroupThreads) void group_tokens_kernel(hf_embedding_backward_args a, TableScratch sc, int range,
-                                                                     unsigned row_bytes, unsigned out_bytes) {
-  extern __shared__ __align__(16) unsigned smem[];   // counters [wave][range], then the hit words
-  __shared__ unsigned wave_part[kGroupWaves], below_part[kGroupWaves];
-  __shared__ unsigned long long zero_rows[kGroupWaves];
-  const I *tokens = static_cast<const I *>(a.tokens);
-  const unsigned n = (unsigned)a.ntokens, vocab = (unsigned)a.vocab;
-  const unsigned pad = a.padding_idx < 0 ? ~0u : (unsigned)a.padding_idx;
-  const unsigned first = blockIdx.x * (unsigned)range, owned = min((unsigned)range, vocab - first);
-  const unsigned tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  unsigned *count = smem + wave * (unsigned)range;
-  unsigned long long *hits = reinterpret_cast<unsigned long long *>(smem + ((kGroupWaves * (unsigned)range + 1u) & ~1u)) + wave * kHitWords;
+// Entry i of the list in hand: of the tokens themselves for the first digit ({i, ~0} for one outside the table or equal to
+// padding_idx), of the list that the digit before left for the others.
+template <class I, bool FIRST>
+__device__ __forceinline__ uint2 list_entry(const hf_embedding_backward_args &a, const uint2 *in, unsigned i, unsigned n) {
+  if (i >= n) return make_uint2(0, ~0u);
+  if constexpr (!FIRST) {
+    return in[i];
+  } else {
+    unsigned lo, hi = 0;
+    if constexpr (sizeof(I) == 8) {
+      const uint2 t = static_cast<const uint2 *>(a.tokens)[i];
+      lo = t.x;
+      hi = t.y;
+    } else {
+      lo = static_cast<const unsigned *>(a.tokens)[i];
+    }
+    const bool used = hi == 0 && lo < (unsigned)a.vocab && (a.padding_idx < 0 || lo != (unsigned)a.padding_idx);
+    return make_uint2(i, used ? lo : ~0u);
+  }
+}
 
-  for (unsigned i = lane; i < (unsigned)range; i += 64) count[i] = 0;   // a wave's counters are its own: no barrier
-
-  const unsigned loads = (n + 63u) / 64u, per = (loads + kGroupWaves - 1) / kGroupWaves;
-  const unsigned from = min(wave * per, loads), to = min(from + per, loads);
-  unsigned below = 0;
-  constexpr int U = 8;   // loads in flight
-  for (unsigned l = from; l < to; l += U) {
-    unsigned key[U];
+// Workgroups [0, tiles): how often each value of the digit occurs in a tile; the first digit's launch notes an owner of
+// every token on the way.  Behind them: rows of zeros (of the other digits' launches).
+template <class I, bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void count_digits_kernel(hf_embedding_backward_args a, TableScratch sc, const uint2 *in, int shift,
+                                                                    int bits, ZeroRows z) {
+  __shared__ unsigned count[kMaxBuckets];
+  const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  if (FIRST && blockIdx.x == 0 && tid == 0) sc.state[1] = 0;
+  if (blockIdx.x >= sc.tiles) {
+    if constexpr (!FIRST) write_zero_rows<I>(a, sc.owner, z, blockIdx.x - sc.tiles);
+    return;
+  }
+  const unsigned buckets = 1u << bits, n = FIRST ? (unsigned)a.ntokens : sc.state[0];
+  for (unsigned b = tid; b < buckets; b += kSortThreads) count[b] = 0;
+  __syncthreads();
+  const unsigned from = blockIdx.x * sc.tile, to = min(from + sc.tile, n);
+  for (unsigned step = from; step < to; step += kSortStep) {
+    unsigned key[kSortKeys];
 #pragma unroll
-    for (int u = 0; u < U; u++) key[u] = l + u < to ? token_key(tokens, (l + u) * 64u + lane, n, vocab, pad) : ~0u;
-    unsigned found = 0;
+    for (int u = 0; u < kSortKeys; u++) key[u] = list_entry<I, FIRST>(a, in, step + (wave * kSortKeys + u) * 64u + lane, to).y;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      below += key[u] < first;
-      const unsigned t = key[u] - first;
-      const unsigned long long mine = __ballot(t < owned);   // (an unusable key is at least 2^31 off)
-      if (mine) {
-        found |= 1u << u;
-        const unsigned t0 = __builtin_amdgcn_readlane(t, __builtin_ctzll(mine));
-        const unsigned long long same = __ballot(t == t0) & mine;
-        if (same == mine) {                      // one token (a run of padding): one addition, not 64 to one address
-          if (lane == 0) atomicAdd(&count[t0], (unsigned)__builtin_popcountll(mine));
-        } else if ((mine >> lane) & 1u) {
-          atomicAdd(&count[t], 1u);
-        }
+    for (int u = 0; u < kSortKeys; u++) {
+      if (FIRST && key[u] != ~0u) sc.owner[key[u]] = step + (wave * kSortKeys + u) * 64u + lane;   // any of them will do
+      const unsigned d = (key[u] >> shift) & (buckets - 1);
+      const unsigned long long used = __ballot(key[u] != ~0u);
+      if (!used) continue;
+      const unsigned d0 = (unsigned)__builtin_amdgcn_readlane((int)d, __builtin_ctzll(used));
+      if ((__ballot(d == d0) & used) == used) {   // a run of one token: one addition, not 64 to one address
+        if (lane == 0) atomicAdd(&count[d0], (unsigned)__builtin_popcountll(used));
+      } else if (key[u] != ~0u) {
+        atomicAdd(&count[d], 1u);
       }
     }
-    const unsigned at = l - from;                // U divides 64: the flags of one trip fall into one word
-    if (lane == 0 && at < 64u * kHitWords) {
-      const unsigned long long bits = (unsigned long long)found << (at & 63u);
-      hits[at >> 6] = (at & 63u) ? hits[at >> 6] | bits : bits;
+  }
+  __syncthreads();
+  for (unsigned b = tid; b < buckets; b += kSortThreads) sc.counts[blockIdx.x * buckets + b] = count[b];
+}
+
+// Workgroups [0, tiles): every entry of a tile to its place, behind all entries of smaller digits and all equal ones before
+// it.  Where the equal ones of other tiles end is summed from their counts; inside the tile a wave numbers its equal
+// entries with ballots, bit by bit of the digit, and the waves follow each other.  Behind them: rows of zeros.
+template <class I, bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void place_digits_kernel(hf_embedding_backward_args a, TableScratch sc, const uint2 *in, uint2 *out,
+                                                                    int shift, int bits, ZeroRows z) {
+  __shared__ unsigned count[kSortWaves][kMaxBuckets], base[kMaxBuckets], scan[kSortWaves];
+  const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  if (blockIdx.x >= sc.tiles) {
+    write_zero_rows<I>(a, sc.owner, z, blockIdx.x - sc.tiles);
+    return;
+  }
+  const unsigned buckets = 1u << bits;
+  constexpr int kOwn = kMaxBuckets / kSortThreads;   // buckets 2 tid and 2 tid + 1 are this thread's
+  unsigned before[kOwn] = {0, 0}, total[kOwn] = {0, 0};
+  if (tid * kOwn < buckets) {   // (one bit: two buckets)
+#pragma unroll 8
+    for (unsigned t = 0; t < sc.tiles; t++) {
+      const uint2 c = *reinterpret_cast<const uint2 *>(sc.counts + t * buckets + tid * kOwn);
+      before[0] += t < blockIdx.x ? c.x : 0;
+      before[1] += t < blockIdx.x ? c.y : 0;
+      total[0] += c.x;
+      total[1] += c.y;
     }
   }
-  below = (unsigned)__builtin_amdgcn_readfirstlane((int)wave_sum_u32(below));
-  if (lane == 0) below_part[wave] = below;
-  __syncthreads();
-
-  // counts -> first entries: over the waves of one token, then over the tokens
-  unsigned total = 0;
-  if (tid < owned)
-    for (int w = 0; w < kGroupWaves; w++) {
-      const unsigned c = smem[w * range + tid];
-      smem[w * range + tid] = total;
-      total += c;
-    }
-  const unsigned long long zeros = __ballot(tid < owned && total == 0);
-  unsigned upto = total;                         // inclusive sum over the lanes
+  unsigned upto = total[0] + total[1];
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
     const unsigned v = __shfl_up(upto, m);
     if (lane >= (unsigned)m) upto += v;
   }
-  if (lane == 63) wave_part[wave] = upto;
-  if (lane == 0) zero_rows[wave] = zeros;
+  if (lane == 63) scan[wave] = upto;
   __syncthreads();
-  unsigned start = upto - total;
-  for (unsigned w = 0; w < kGroupWaves; w++) {
-    start += below_part[w];
-    if (w < wave) start += wave_part[w];
+  unsigned all = 0;
+#pragma unroll
+  for (unsigned w = 0; w < kSortWaves; w++) {
+    if (w < wave) upto += scan[w];
+    all += scan[w];
   }
-  if (tid < owned) {
-    sc.starts[first + tid] = start;
-    if (first + tid == vocab - 1) sc.starts[vocab] = start + total;
-    for (int w = 0; w < kGroupWaves; w++) smem[w * range + tid] += start;
+  if (tid * kOwn < buckets) {
+    base[tid * kOwn] = upto - total[0] - total[1] + before[0];
+    base[tid * kOwn + 1] = upto - total[1] + before[1];
   }
-  if (blockIdx.x == 0 && tid == 0) *sc.nlong = 0;
+  if (FIRST && blockIdx.x == 0 && tid == 0) sc.state[0] = all;
 
-  __syncthreads();   // the first entries of all waves' counters
-
-  // rows of zeros, a wave a row
-  auto write_zeros = [&] {
-    unsigned char *out = static_cast<unsigned char *>(a.dweight);
-    for (unsigned r = wave; r < owned; r += kGroupWaves) {
-      if (!((zero_rows[r >> 6] >> (r & 63u)) & 1ull)) continue;
-      unsigned char *row = out + (size_t)(first + r) * (size_t)a.dweight_stride * out_bytes;
-      if (row_bytes >= 16) {
-        const unsigned slots = (row_bytes + 15u) / 16u;
-        for (unsigned j = lane; j < slots; j += 64) store_vec<unsigned short, 8>(reinterpret_cast<unsigned short *>(row + min(j * 16u, row_bytes - 16u)), (vec_t<unsigned short, 8>)(0));
-      } else if (lane * 2u < row_bytes) {
-        reinterpret_cast<unsigned short *>(row)[lane] = 0;
+  const unsigned n = FIRST ? (unsigned)a.ntokens : all;
+  const unsigned from = blockIdx.x * sc.tile, to = min(from + sc.tile, n);
+  for (unsigned step = from; step < to; step += kSortStep) {
+    uint2 entry[kSortKeys];
+#pragma unroll
+    for (int u = 0; u < kSortKeys; u++) entry[u] = list_entry<I, FIRST>(a, in, step + (wave * kSortKeys + u) * 64u + lane, to);
+    for (unsigned b = lane; b < buckets; b += 64) count[wave][b] = 0;   // a wave's counters are its own
+    unsigned rank[kSortKeys];
+#pragma unroll
+    for (int u = 0; u < kSortKeys; u++) {
+      const unsigned d = (entry[u].y >> shift) & (buckets - 1);
+      const bool used = entry[u].y != ~0u;
+      unsigned long long same = __ballot(used);
+      for (int b = 0; b < bits; b++) {
+        const bool one = (d >> b) & 1u;
+        const unsigned long long ones = __ballot(one);
+        same &= one ? ones : ~ones;
+      }
+      rank[u] = 0;
+      if (used) {
+        const int leader = __builtin_ctzll(same);
+        if ((int)lane == leader) rank[u] = atomicAdd(&count[wave][d], (unsigned)__builtin_popcountll(same));
+        rank[u] = (unsigned)__shfl((int)rank[u], leader) + (unsigned)__builtin_popcountll(same & ((1ull << lane) - 1ull));
       }
     }
-  };
-  // second look, at the loads that held a token of the range
-  auto place = [&] {
-    const unsigned bits = 32u - (unsigned)__builtin_clz(max(owned, 2u) - 1u);
-    const bool remembered = per <= 64u * kHitWords;
-    for (unsigned g = 0; g * 64u < to - from; g++) {
-      unsigned long long todo = ~0ull;
-      if (remembered) {
-        const unsigned long long h = hits[g];
-        todo = ((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(h >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)h);
-      } else if (to - from - g * 64u < 64u) {
-        todo = (1ull << (to - from - g * 64u)) - 1ull;
+    __syncthreads();
+    for (unsigned b = tid; b < buckets; b += kSortThreads) {   // counts -> first places; the tile's next step follows
+      unsigned at = base[b];
+#pragma unroll
+      for (int w = 0; w < kSortWaves; w++) {
+        const unsigned c = count[w][b];
+        count[w][b] = at;
+        at += c;
       }
-      while (todo) {
-        constexpr int B = 4;
-        unsigned key[B], pos[B];
-  #pragma unroll
-        for (int b = 0; b < B; b++) {
-          pos[b] = ~0u;
-          if (todo) {
-            pos[b] = (from + g * 64u + (unsigned)__builtin_ctzll(todo)) * 64u + lane;
-            todo &= todo - 1;
-          }
-          key[b] = pos[b] == ~0u ? ~0u : token_key(tokens, pos[b], n, vocab, pad);
-        }
-  #pragma unroll
-        for (int b = 0; b < B; b++) {
-          const unsigned t = key[b] - first;
-          const bool in = t < owned;
-          unsigned long long same = __ballot(in);
-          if (!same) continue;
-          for (unsigned bit = 0; bit < bits; bit++) {   // the lanes with my token
-            const bool one = (t >> bit) & 1u;
-            const unsigned long long ones = __ballot(in && one);
-            same &= one ? ones : ~ones;
-          }
-          if (in) {
-            const int leader = __builtin_ctzll(same);
-            unsigned at = 0;
-            if ((int)lane == leader) at = atomicAdd(&count[t], (unsigned)__builtin_popcountll(same));
-            at = (unsigned)__shfl((int)at, leader);
-            at += (unsigned)__builtin_popcountll(same & ((1ull << lane) - 1ull));
-            sc.order[at] = make_uint2(pos[b], key[b]);
-          }
-        }
-      }
+      base[b] = at;
     }
-  };
-  if (wave & 1u) {   // half the waves store while the others look
-    write_zeros();
-    place();
-  } else {
-    place();
-    write_zeros();
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kSortKeys; u++)
+      if (entry[u].y != ~0u) out[count[wave][(entry[u].y >> shift) & (buckets - 1)] + rank[u]] = entry[u];
+    __syncthreads();   // (a faster wave clears its own counters only, but `base` and the places above are everyone's)
   }
 }
 
-// A group of `lanes` lanes sums the rows of one chunk of `order` over one tile of columns (lanes * VPT slots).  A token
-// with at most `chunk` rows belongs to the chunk it starts in, which follows it to its end; a token with more is shared:
-// every chunk sums its own part of it.
-template <class T, class O, int VEC, int VPT, bool WIDE>
-__global__ __launch_bounds__(256) void sum_rows_kernel(hf_embedding_backward_args a, TableScratch sc, int lanes_log2, int tiles) {
+// First entry of [lo, hi) whose token is larger than `id` (hi if there is none); the list is sorted.
+__device__ __forceinline__ unsigned first_above(const uint2 *order, unsigned lo, unsigned hi, unsigned id) {
+  while (lo < hi) {
+    const unsigned mid = (lo + hi) / 2;
+    if (order[mid].y > id) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+// A group of `lanes` lanes sums the rows of one chunk of `order` over one tile of columns (`lanes` slots).  A token whose rows
+// cross one chunk boundary at most belongs to the chunk it starts in, which follows it to its end; a token that crosses
+// more is shared: every chunk sums its own part of it.
+template <class T, class O, int VEC, bool WIDE>
+__global__ __launch_bounds__(256) void sum_rows_kernel(hf_embedding_backward_args a, TableScratch sc, int lanes_log2, unsigned tiles) {
   const int lanes = WIDE ? 64 : 1 << lanes_log2;
   const unsigned global = blockIdx.x * 256u + threadIdx.x;
-  unsigned group = WIDE ? (unsigned)__builtin_amdgcn_readfirstlane((int)(global >> 6)) : global >> lanes_log2;
+  const unsigned group = WIDE ? (unsigned)__builtin_amdgcn_readfirstlane((int)(global >> 6)) : global >> lanes_log2;
   const int lane = (int)(threadIdx.x & (unsigned)(lanes - 1));
-  const int c = (int)(group / (unsigned)tiles), tile = (int)(group % (unsigned)tiles);
-  const unsigned used = sc.starts[a.vocab];
-  const unsigned k0 = (unsigned)c * (unsigned)sc.chunk;
+  const unsigned c = group / tiles;
+  const int tile = (int)(group % tiles);
+  const unsigned used = sc.state[0], k0 = c * sc.chunk;
   if (c >= sc.nchunks || k0 >= used) return;
-  const unsigned k1 = min(k0 + (unsigned)sc.chunk, used);
-  const unsigned id0 = sc.order[k0].y, idl = sc.order[k1 - 1].y;
-  const unsigned s0 = sc.starts[id0], e0 = sc.starts[id0 + 1], sl = sc.starts[idl], el = sc.starts[idl + 1];
-  const bool long0 = e0 - s0 > (unsigned)sc.chunk && s0 < k0;    // continues a shared token
-  const bool longl = el - sl > (unsigned)sc.chunk && sl >= k0;   // a shared token starts here
-  const unsigned begin = (s0 < k0 && !long0) ? e0 : k0;          // the end of an earlier chunk's token is that chunk's
-  const unsigned end = (el - sl > (unsigned)sc.chunk) ? k1 : (sl >= k0 ? el : min(el, k1));
-  if (longl && tile == 0 && lane == 0) sc.longs[atomicAdd(sc.nlong, 1u)] = (unsigned)c;   // in any order: each is joined by itself
+  const uint2 *order = sc.order;
+  const unsigned k1 = min(k0 + sc.chunk, used);
+  const unsigned id0 = order[k0].y, idl = order[k1 - 1].y;
+  const bool cont0 = k0 > 0 && order[k0 - 1].y == id0;                       // started in a chunk before
+  const bool crosses = k1 < used && order[k1].y == idl;                      // goes on in the chunk behind
+  const bool starts = !(cont0 && idl == id0);
+  const bool shared0 = cont0 && ((crosses && idl == id0) || (k0 > sc.chunk && order[k0 - sc.chunk - 1].y == id0));
+  const bool sharedl = starts && crosses && k1 + sc.chunk < used && order[k1 + sc.chunk].y == idl;
+  const unsigned begin = cont0 && !shared0 ? first_above(order, k0, k1, id0) : k0;   // the rest of that token is the other chunk's
+  const unsigned end = starts && crosses && !sharedl ? first_above(order, k1, min(k1 + sc.chunk, used), idl) : k1;
+  if (tile == 0 && lane == 0) {
+    if (sharedl) sc.shared[atomicAdd(&sc.state[1], 1u)] = c;   // in any order: each is joined by itself
+    if (shared0 && !(crosses && idl == id0)) sc.last[id0] = c;
+  }
 
   const int cols = (int)a.cols, slots = row_slots<VEC>(cols);
-  int col[VPT], slot[VPT];
+  const int slot = tile * lanes + lane, col = slot_column<VEC>(min(slot, slots - 1), cols);   // (lanes behind the row store nothing)
+  const T *dy = static_cast<const T *>(a.dy) + col;
+  float acc[VEC];
 #pragma unroll
-  for (int v = 0; v < VPT; v++) {
-    slot[v] = (tile * VPT + v) * lanes + lane;
-    col[v] = slot_column<VEC>(min(slot[v], slots - 1), cols);   // lanes behind the row repeat its last slot and store nothing
-  }
-  const T *dy = static_cast<const T *>(a.dy);
-  float acc[VPT][VEC];
-#pragma unroll
-  for (int v = 0; v < VPT; v++)
-#pragma unroll
-    for (int e = 0; e < VEC; e++) acc[v][e] = 0.0f;
+  for (int e = 0; e < VEC; e++) acc[e] = 0.0f;
 
-  constexpr int U = 4;
-  for (unsigned k = begin; k < end; k += U) {
-    uint2 entry[U];
-    unsigned next;
+  // the sum of a token's rows of this chunk: to its row of the gradient, or to the parts of a shared token
+  auto put = [&](unsigned id) {
+    const bool part0 = shared0 && id == id0, partl = sharedl && id == idl;
+    if (slot < slots) {
+      if (part0 || partl) {
+        store_vec<float, VEC>(sc.partial + (((size_t)c * 2 + (part0 ? 0 : 1)) * (size_t)slots + (size_t)slot) * VEC, round_vec<float, VEC>(acc));
+      } else {
+        float s[VEC];
 #pragma unroll
-    for (int u = 0; u < U; u++) entry[u] = sc.order[min(k + u, end - 1)];
-    next = sc.order[min(k + U, end - 1)].y;
-    vec_t<T, VEC> row[U][VPT];
+        for (int e = 0; e < VEC; e++) s[e] = acc[e] * a.scale;
+        store_vec<O, VEC>(static_cast<O *>(a.dweight) + (size_t)id * (size_t)a.dweight_stride + col, round_vec<O, VEC>(s));
+      }
+    }
 #pragma unroll
-    for (int u = 0; u < U; u++)
+    for (int e = 0; e < VEC; e++) acc[e] = 0.0f;
+  };
+  auto add = [&](const vec_t<T, VEC> &row) {
 #pragma unroll
-      for (int v = 0; v < VPT; v++) row[u][v] = load_vec<T, VEC>(dy + (size_t)entry[u].x * (size_t)a.dy_stride + col[v]);
+    for (int e = 0; e < VEC; e++) acc[e] += elem<T, VEC>(row, e);
+  };
+  constexpr int U = 4;   // rows on their way at once (twice that in a whole wave)
+  if constexpr (WIDE) {
+    // 64 entries at a time in the wave's lanes: a row's address is one v_readlane away, and the tokens' last rows are the
+    // bits of one ballot.  The next U rows are on their way while U are added.
+    for (unsigned base = begin; base < end; base += 64) {
+      const int m = (int)min(64u, end - base);
+      const uint2 mine = order[min(base + (unsigned)lane, end - 1)];
+      const unsigned behind = order[min(base + (unsigned)lane + 1, end - 1)].y;
+      const unsigned long long lasts = __ballot(behind != mine.y || base + (unsigned)lane + 1 >= end);
+      auto fetch = [&](vec_t<T, VEC> (&row)[U], int at) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      if (k + u < end) {
+        for (int u = 0; u < U; u++)
+          row[u] = load_vec_stream<T, VEC>(dy + (size_t)(unsigned)__builtin_amdgcn_readlane((int)mine.x, min(at + u, m - 1)) * (size_t)a.dy_stride);
+      };
+      auto take = [&](const vec_t<T, VEC> (&row)[U], int at) {
 #pragma unroll
-        for (int v = 0; v < VPT; v++)
-#pragma unroll
-          for (int e = 0; e < VEC; e++) acc[v][e] += elem<T, VEC>(row[u][v], e);
-        const unsigned id = entry[u].y;
-        if (k + u + 1 == end || id != (u + 1 < U ? entry[u + 1 < U ? u + 1 : u].y : next)) {   // the token's last row here
-          const bool part0 = long0 && id == id0, partl = longl && id == idl;
-#pragma unroll
-          for (int v = 0; v < VPT; v++) {
-            if (slot[v] < slots) {
-              if (part0 || partl) {
-                float *p = sc.partial + ((size_t)c * 2 + (part0 ? 0 : 1)) * ((size_t)slots * VEC) + (size_t)slot[v] * VEC;
-                store_vec<float, VEC>(p, round_vec<float, VEC>(acc[v]));
-              } else {
-                float s[VEC];
-#pragma unroll
-                for (int e = 0; e < VEC; e++) s[e] = acc[v][e] * a.scale;
-                store_vec<O, VEC>(static_cast<O *>(a.dweight) + (size_t)id * (size_t)a.dweight_stride + col[v], round_vec<O, VEC>(s));
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < VEC; e++) acc[v][e] = 0.0f;
+        for (int u = 0; u < U; u++) {
+          if (at + u < m) {
+            add(row[u]);
+            if ((lasts >> (at + u)) & 1ull) put((unsigned)__builtin_amdgcn_readlane((int)mine.y, at + u));
           }
+        }
+      };
+      vec_t<T, VEC> one[U], two[U];
+      fetch(one, 0);
+      for (int at = 0; at < m; at += 2 * U) {
+        fetch(two, at + U);
+        take(one, at);
+        if (at + 2 * U < m) fetch(one, at + 2 * U);
+        take(two, at + U);
+      }
+    }
+  } else {
+    for (unsigned k = begin; k < end; k += U) {
+      uint2 entry[U + 1];
+#pragma unroll
+      for (int u = 0; u <= U; u++) entry[u] = order[min(k + u, end - 1)];
+      vec_t<T, VEC> row[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) row[u] = load_vec_stream<T, VEC>(dy + (size_t)entry[u].x * (size_t)a.dy_stride);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        if (k + u < end) {
+          add(row[u]);
+          if (k + u + 1 == end || entry[u].y != entry[u + 1].y) put(entry[u].y);
         }
       }
     }
@@ -299,16 +347,16 @@ __global__ __launch_bounds__(256) void sum_rows_kernel(hf_embedding_backward_arg
 // and their sums are added in the order of the waves.
 constexpr int kJoinWaves = 16;
 template <class O, int VEC>
-__global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(hf_embedding_backward_args a, TableScratch sc, int tiles) {
+__global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(hf_embedding_backward_args a, TableScratch sc, unsigned tiles) {
   __shared__ float sums[kJoinWaves][64 * VEC];
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   const int cols = (int)a.cols, slots = row_slots<VEC>(cols);
-  const unsigned items = *sc.nlong * (unsigned)tiles;
-  for (unsigned item = blockIdx.x; item < items; item += gridDim.x) {
-    const unsigned c = sc.longs[item / (unsigned)tiles];
-    const int slot = (int)(item % (unsigned)tiles) * 64 + lane;
-    const unsigned id = sc.order[min((c + 1) * (unsigned)sc.chunk, sc.starts[a.vocab]) - 1].y;
-    const unsigned last = (sc.starts[id + 1] - 1) / (unsigned)sc.chunk;   // the chunk its last row is in
+  const unsigned long long items = (unsigned long long)sc.state[1] * tiles;
+  for (unsigned long long item = blockIdx.x; item < items; item += gridDim.x) {
+    const unsigned c = sc.shared[item / tiles];
+    const int slot = (int)(item % tiles) * 64 + lane;
+    const unsigned id = sc.order[(c + 1) * sc.chunk - 1].y;   // (a shared token fills the chunk behind: this one is full)
+    const unsigned last = sc.last[id];
     const size_t width = (size_t)slots * VEC;
     const float *p = sc.partial + (size_t)min(slot, slots - 1) * VEC;
     float acc[VEC];
@@ -337,14 +385,14 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(hf_embedding
   }
 }
 
-// How the launches are cut: columns into slots and tiles, sorted entries into chunks.
-struct TablePlan {
-  int vec, vpt, lanes_log2, tiles, chunk, nchunks, range, slots;
-  unsigned ranges;
-  size_t order_at, longs_at, partial_at, bytes;   // starts and nlong are at the front
-};
+constexpr int kMaxChunk = 64, kSumWaves = 16;   // entries of a chunk at most; waves a CU should have at least
 
-size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
+// How the launches are cut: columns into slots and tiles, sorted entries into chunks, the token's bits into digits.
+struct TablePlan {
+  int vec, lanes_log2, slots, passes, digit_bits, zero_log2;
+  unsigned col_tiles, chunk, nchunks, tile, tiles;
+  size_t owner_at, last_at, shared_at, counts_at, order_at, other_at, partial_at, bytes;   // the state is at the front
+};
 
 TablePlan plan_table(const hf_embedding_backward_args &a, int cus) {
   TablePlan p;
@@ -354,39 +402,88 @@ TablePlan plan_table(const hf_embedding_backward_args &a, int cus) {
   p.lanes_log2 = 6;
   while (p.lanes_log2 > 0 && (1 << (p.lanes_log2 - 1)) >= p.slots) p.lanes_log2--;
   const int lanes = 1 << p.lanes_log2;
-  p.vpt = p.slots > 64 ? 2 : 1;
-  p.tiles = (p.slots + lanes * p.vpt - 1) / (lanes * p.vpt);
-  p.chunk = 64;
-  while (p.chunk > 8 && a.ntokens / p.chunk * p.tiles * lanes < (int64_t)cus * 16 * 64) p.chunk /= 2;
-  while (a.ntokens / p.chunk * p.tiles * lanes >= (int64_t)1 << 31) p.chunk *= 2;   // lanes are numbered in 32 bits
-  p.nchunks = (int)((a.ntokens + p.chunk - 1) / p.chunk);
-  p.range = (int)std::min<int64_t>(kMaxRange, (a.vocab + cus - 1) / cus);
-  p.ranges = (unsigned)((a.vocab + p.range - 1) / p.range);
-  size_t at = round16(((size_t)a.vocab + 2) * sizeof(unsigned));
-  p.order_at = at;
-  at = round16(at + (size_t)a.ntokens * sizeof(uint2));
-  p.longs_at = at;
-  at = round16(at + (size_t)p.nchunks * sizeof(unsigned));
-  p.partial_at = at;
-  p.bytes = round16(at + (size_t)p.nchunks * 2 * (size_t)p.slots * (size_t)p.vec * sizeof(float));
+  p.col_tiles = (unsigned)((p.slots + lanes - 1) / lanes);
+  p.chunk = kMaxChunk;
+  while (p.chunk > 8 && a.ntokens / p.chunk * p.col_tiles * lanes < (int64_t)cus * kSumWaves * 64) p.chunk /= 2;
+  while (a.ntokens / p.chunk * p.col_tiles * lanes >= (int64_t)1 << 31) p.chunk *= 2;   // lanes are numbered in 32 bits
+  p.nchunks = (unsigned)((a.ntokens + p.chunk - 1) / p.chunk);
+  int bits = 1;
+  while (((int64_t)1 << bits) < a.vocab) bits++;
+  p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
+  p.digit_bits = (bits + p.passes - 1) / p.passes;
+  const int64_t steps = (a.ntokens + kSortStep - 1) / kSortStep;
+  p.tile = (unsigned)((steps + kSortTiles - 1) / kSortTiles * kSortStep);
+  p.tiles = p.tile ? (unsigned)((a.ntokens + p.tile - 1) / p.tile) : 0;
+  const int64_t row_bytes = a.cols * (a.out_type == HF_F32 ? 4 : 2);
+  p.zero_log2 = 0;   // lanes to a row of zeros: as many as it has 16-byte stores, a workgroup at most
+  while (p.zero_log2 < 8 && ((int64_t)16 << p.zero_log2) < row_bytes) p.zero_log2++;
+  while (p.zero_log2 > 0 && (a.vocab << p.zero_log2) >= (int64_t)1 << 31) p.zero_log2--;
+  size_t at = 16;
+  auto take = [&at](size_t bytes) {
+    const size_t here = at;
+    at = (at + bytes + 15) & ~(size_t)15;
+    return here;
+  };
+  p.owner_at = take((size_t)a.vocab * sizeof(unsigned));
+  p.last_at = take((size_t)a.vocab * sizeof(unsigned));
+  p.shared_at = take((size_t)p.nchunks * sizeof(unsigned));
+  p.counts_at = take(((size_t)p.tiles << p.digit_bits) * sizeof(unsigned));
+  p.order_at = take((size_t)a.ntokens * sizeof(uint2));
+  p.other_at = take(p.passes > 1 ? (size_t)a.ntokens * sizeof(uint2) : 0);
+  p.partial_at = take((size_t)p.nchunks * 2 * (size_t)p.slots * (size_t)p.vec * sizeof(float));
+  p.bytes = at;
   return p;
 }
 
 template <class T, class O, int VEC>
 hipError_t sum_tokens(const hf_embedding_backward_args &a, const TablePlan &p, const TableScratch &sc, int cus, hipStream_t s) {
-  const unsigned long long blocks = ((((unsigned long long)p.nchunks * (unsigned)p.tiles) << p.lanes_log2) + 255) / 256;
-  if (p.vpt == 2)
-    hipLaunchKernelGGL((sum_rows_kernel<T, O, VEC, 2, true>), dim3((unsigned)blocks), dim3(256), 0, s, a, sc, 6, p.tiles);
-  else if (p.lanes_log2 == 6)
-    hipLaunchKernelGGL((sum_rows_kernel<T, O, VEC, 1, true>), dim3((unsigned)blocks), dim3(256), 0, s, a, sc, 6, p.tiles);
+  const unsigned long long sums = ((((unsigned long long)p.nchunks * p.col_tiles) << p.lanes_log2) + 255) / 256;
+  const dim3 grid((unsigned)sums);
+  if (sums == 0) return hipSuccess;
+  if (p.lanes_log2 == 6)
+    hipLaunchKernelGGL((sum_rows_kernel<T, O, VEC, true>), grid, dim3(256), 0, s, a, sc, 6, p.col_tiles);
   else
-    hipLaunchKernelGGL((sum_rows_kernel<T, O, VEC, 1, false>), dim3((unsigned)blocks), dim3(256), 0, s, a, sc, p.lanes_log2, p.tiles);
+    hipLaunchKernelGGL((sum_rows_kernel<T, O, VEC, false>), grid, dim3(256), 0, s, a, sc, p.lanes_log2, p.col_tiles);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  const int join_tiles = (p.slots + 63) / 64;
-  const unsigned grid = (unsigned)std::min<unsigned long long>((unsigned long long)p.nchunks * (unsigned)join_tiles, (unsigned long long)cus * 4);
-  hipLaunchKernelGGL((join_rows_kernel<O, VEC>), dim3(grid), dim3(64 * kJoinWaves), 0, s, a, sc, join_tiles);
+  if (e != hipSuccess || p.nchunks < 3) return e;   // a shared token crosses two chunk boundaries
+  const unsigned join_tiles = (unsigned)(p.slots + 63) / 64;
+  const unsigned joins = (unsigned)std::min<unsigned long long>((unsigned long long)p.nchunks * join_tiles, (unsigned long long)cus * 4);
+  hipLaunchKernelGGL((join_rows_kernel<O, VEC>), dim3(joins), dim3(64 * kJoinWaves), 0, s, a, sc, join_tiles);
   return hipGetLastError();
+}
+
+template <class I>
+hipError_t sort_tokens(const hf_embedding_backward_args &a, const TablePlan &p, const TableScratch &sc, const ZeroRows &all, hipStream_t s) {
+  // the rows of zeros are shared evenly among the launches behind the first, which finds out what they are
+  const unsigned parts = 2u * (unsigned)p.passes - 1u;
+  ZeroRows z = {0, 0, all.lanes_log2, all.element};
+  unsigned part = 0;
+  auto zero_blocks = [&] {
+    z.row = (unsigned)((unsigned long long)all.rows * part / parts);
+    z.rows = (unsigned)((unsigned long long)all.rows * (part + 1) / parts) - z.row;
+    part++;
+    return (unsigned)((((unsigned long long)z.rows << z.lanes_log2) + 255) / 256);
+  };
+  // the lists change places with every digit, so that the last one fills sc.order
+  uint2 *in = nullptr, *out = p.passes % 2 ? sc.order : sc.other;
+  for (int pass = 0; pass < p.passes; pass++) {
+    const int shift = pass * p.digit_bits;
+    if (pass == 0)
+      hipLaunchKernelGGL((count_digits_kernel<I, true>), dim3(std::max(p.tiles, 1u)), dim3(kSortThreads), 0, s, a, sc, in, shift, p.digit_bits, z);
+    else if (const unsigned blocks = p.tiles + zero_blocks())
+      hipLaunchKernelGGL((count_digits_kernel<I, false>), dim3(blocks), dim3(kSortThreads), 0, s, a, sc, in, shift, p.digit_bits, z);
+    if (const unsigned blocks = p.tiles + zero_blocks()) {
+      if (pass == 0)
+        hipLaunchKernelGGL((place_digits_kernel<I, true>), dim3(blocks), dim3(kSortThreads), 0, s, a, sc, in, out, shift, p.digit_bits, z);
+      else
+        hipLaunchKernelGGL((place_digits_kernel<I, false>), dim3(blocks), dim3(kSortThreads), 0, s, a, sc, in, out, shift, p.digit_bits, z);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    in = out;
+    out = out == sc.order ? sc.other : sc.order;
+  }
+  return hipSuccess;
 }
 
 template <class T>
@@ -394,21 +491,21 @@ hipError_t embed_backward(const hf_embedding_backward_args &a, int cus, hipStrea
   const TablePlan p = plan_table(a, cus);
   unsigned char *ws = static_cast<unsigned char *>(a.workspace);
   TableScratch sc;
-  sc.starts = reinterpret_cast<unsigned *>(ws);
-  sc.nlong = sc.starts + a.vocab + 1;
+  sc.state = reinterpret_cast<unsigned *>(ws);
+  sc.owner = reinterpret_cast<unsigned *>(ws + p.owner_at);
+  sc.last = reinterpret_cast<unsigned *>(ws + p.last_at);
+  sc.shared = reinterpret_cast<unsigned *>(ws + p.shared_at);
+  sc.counts = reinterpret_cast<unsigned *>(ws + p.counts_at);
   sc.order = reinterpret_cast<uint2 *>(ws + p.order_at);
-  sc.longs = reinterpret_cast<unsigned *>(ws + p.longs_at);
+  sc.other = reinterpret_cast<uint2 *>(ws + p.other_at);
   sc.partial = reinterpret_cast<float *>(ws + p.partial_at);
+  sc.tile = p.tile;
+  sc.tiles = p.tiles;
   sc.chunk = p.chunk;
   sc.nchunks = p.nchunks;
-  const unsigned out_bytes = a.out_type == HF_F32 ? 4 : 2;
-  const size_t lds = (((size_t)kGroupWaves * p.range + 1) & ~(size_t)1) * 4 + (size_t)kGroupWaves * kHitWords * 8;
-  if (a.index_type == HF_I64)
-    hipLaunchKernelGGL(group_tokens_kernel<int64_t>, dim3(p.ranges), dim3(kGroupThreads), lds, s, a, sc, p.range, (unsigned)a.cols * out_bytes, out_bytes);
-  else
-    hipLaunchKernelGGL(group_tokens_kernel<int32_t>, dim3(p.ranges), dim3(kGroupThreads), lds, s, a, sc, p.range, (unsigned)a.cols * out_bytes, out_bytes);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.ntokens == 0) return e;
+  const ZeroRows all = {0, (unsigned)a.vocab, p.zero_log2, a.out_type == HF_F32 ? 4u : 2u};
+  const hipError_t e = a.index_type == HF_I64 ? sort_tokens<int64_t>(a, p, sc, all, s) : sort_tokens<int32_t>(a, p, sc, all, s);
+  if (e != hipSuccess) return e;
   if (a.out_type == HF_F32)
     return p.vec == 1 ? sum_tokens<T, float, 1>(a, p, sc, cus, s) : sum_tokens<T, float, kVec<T>>(a, p, sc, cus, s);
   return p.vec == 1 ? sum_tokens<T, T, 1>(a, p, sc, cus, s) : sum_tokens<T, T, kVec<T>>(a, p, sc, cus, s);
