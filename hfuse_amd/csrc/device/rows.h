@@ -86,18 +86,43 @@ __device__ __forceinline__ int slot_repeats(int j, int cols) {
   return max(0, j * N - (cols - N));
 }
 
-// Sum over the 64 lanes, in every lane: a butterfly, so the order of the additions is fixed.
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+// Sum over aligned groups of LANES lanes (a power of two up to 64), in every lane.  The steps inside 16 lanes are DPP moves
+// (quad permutes, mirrors of 8 and of 16: each pairs lanes whose partial sums cover disjoint halves, as an xor would).
+template <int CTRL>
+__device__ __forceinline__ float dpp_move(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (LANES >= 2) v += dpp_move<0xB1>(v);    // quad_perm [1,0,3,2]
+  if constexpr (LANES >= 4) v += dpp_move<0x4E>(v);    // quad_perm [2,3,0,1]
+  if constexpr (LANES >= 8) v += dpp_move<0x141>(v);   // row_half_mirror
+  if constexpr (LANES >= 16) v += dpp_move<0x140>(v);  // row_mirror
+  if constexpr (LANES >= 32) v += __shfl_xor(v, 16);
+  if constexpr (LANES >= 64) v += __shfl_xor(v, 32);
   return v;
 }
 
-__device__ __forceinline__ unsigned wave_sum_u32(unsigned v) {
+// Column slots of a row shared by LANES threads, VPT slots each: thread t has slots t, t + LANES, ...
+template <int VEC, int VPT, int LANES>
+struct RowSlots {
+  int col[VPT];       // first column (threads behind the row repeat its last slot)
+  int skip[VPT];      // elements of the slot that are not this thread's to count: repeats, or all VEC behind the row
+  bool whole[VPT];    // wave-uniform: no lane of the wave skips anything
+  __device__ __forceinline__ RowSlots(int t, int cols) {
+    const int slots = row_slots<VEC>(cols);
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
-  return v;
-}
+    for (int k = 0; k < VPT; k++) {
+      const int j = t + k * LANES;
+      col[k] = slot_column<VEC>(min(j, slots - 1), cols);
+      skip[k] = j < slots ? slot_repeats<VEC>(j, cols) : VEC;
+      whole[k] = __ballot(skip[k] != 0) == 0;
+    }
+  }
+};
+
+// Inputs too large to be in the 256 MB memory-side cache from whatever wrote them are read past the caches.
+inline bool past_caches(size_t bytes) { return bytes > ((size_t)256 << 20); }
 
 // Calls f with a value of the type that `type` (HF_F32 / HF_BF16 / HF_F16) names.
 template <class F>

@@ -1,4 +1,4 @@
-// Layer norm over the last dimension and its gradient.
+// Layer norm over the last dimension.
 #include <algorithm>
 
 #include "device/rows.h"
@@ -7,41 +7,150 @@
 namespace hfuse {
 namespace {
 
-constexpr int kThreads = 256;
 
-// Sum over the workgroup, in every thread.
-__device__ __forceinline__ float block_sum(float v, float *part) {
-  v = wave_sum(v);
-  __syncthreads();   // the slots may still be read for the sum before
-  if ((threadIdx.x & 63u) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0.0f;
+// LANES threads hold a row in registers, VPT slots of 16 bytes each: the row is read once, the mean and then the mean
+// square of the differences come from the registers, and the next row is on its way meanwhile.  A workgroup keeps its
+// weights in registers for all its rows.
+template <class T, class P, int VEC, int VPT, int LANES, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_args a, bool stream) {
+  constexpr int GROUPS = BLOCK / LANES, WAVES = LANES > 64 ? LANES / 64 : 1;
+  constexpr bool kKeep = VPT * VEC * BLOCK <= 16 * 1024;   // weights and biases fit the registers next to two rows
+  __shared__ float part[2][BLOCK / 64];
+  const int cols = (int)a.cols, t = (int)threadIdx.x % LANES, group = (int)threadIdx.x / LANES;
+  const RowSlots<VEC, VPT, LANES> map(t, cols);
+  const P *weight = static_cast<const P *>(a.weight), *bias = static_cast<const P *>(a.bias);
+  auto load_params = [&](int k, vec_t<P, VEC> &w, vec_t<P, VEC> &b) {
+    w = weight ? load_vec<P, VEC>(weight + map.col[k]) : (vec_t<P, VEC>)(P)1.0f;
+    b = bias ? load_vec<P, VEC>(bias + map.col[k]) : (vec_t<P, VEC>)(P)0.0f;
+  };
+  vec_t<P, VEC> w[kKeep ? VPT : 1], b[kKeep ? VPT : 1];
+  if constexpr (kKeep) {
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; w++) v += part[w];
-  return v;
+    for (int k = 0; k < VPT; k++) load_params(k, w[k], b[k]);
+  }
+  const float inv = 1.0f / (float)cols;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  auto sum_row = [&](float v, int which) {
+    v = lanes_sum<(LANES < 64 ? LANES : 64)>(v);
+    if constexpr (LANES > 64) {
+      if ((threadIdx.x & 63u) == 0) part[which][threadIdx.x >> 6] = v;
+      __syncthreads();   // two slots in turn: a slot is written again only behind the other one's barrier
+      v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < WAVES; i++) v += part[which][group * WAVES + i];
+    }
+    return v;
+  };
+  vec_t<T, VEC> next[VPT];
+  auto fetch = [&](int64_t row) {
+    const T *x = static_cast<const T *>(a.x) + min(row, a.rows - 1) * a.x_stride;
+#pragma unroll
+    for (int k = 0; k < VPT; k++) next[k] = stream ? load_vec_stream<T, VEC>(x + map.col[k]) : load_vec<T, VEC>(x + map.col[k]);
+  };
+  fetch((int64_t)blockIdx.x * GROUPS + group);
+  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < a.rows; base += step) {   // all groups of a workgroup make the same trips
+    const int64_t row = base + group;
+    vec_t<T, VEC> x[VPT];
+#pragma unroll
+    for (int k = 0; k < VPT; k++) x[k] = next[k];
+    if (base + step < a.rows) fetch(row + step);
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < VPT; k++) {
+      if (map.whole[k]) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) s += elem<T, VEC>(x[k], e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) s += e >= map.skip[k] ? elem<T, VEC>(x[k], e) : 0.0f;
+      }
+    }
+    const float mean = sum_row(s, 0) * inv;
+    s = 0.0f;
+    float d[VPT][VEC];
+#pragma unroll
+    for (int k = 0; k < VPT; k++) {
+#pragma unroll
+      for (int e = 0; e < VEC; e++) d[k][e] = elem<T, VEC>(x[k], e) - mean;
+      if (map.whole[k]) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) s += d[k][e] * d[k][e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) s += e >= map.skip[k] ? d[k][e] * d[k][e] : 0.0f;
+      }
+    }
+    const float rstd = 1.0f / sqrtf(sum_row(s, 1) * inv + a.eps);
+    if (row < a.rows) {
+      T *y = static_cast<T *>(a.y) + row * a.y_stride;
+#pragma unroll
+      for (int k = 0; k < VPT; k++) {
+        if (map.skip[k] == VEC) continue;
+        vec_t<P, VEC> wk, bk;
+        if constexpr (kKeep) {
+          wk = w[k];
+          bk = b[k];
+        } else {
+          load_params(k, wk, bk);
+        }
+        float out[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) out[e] = d[k][e] * rstd * elem<P, VEC>(wk, e) + elem<P, VEC>(bk, e);
+        store_vec_stream<T, VEC>(y + map.col[k], round_vec<T, VEC>(out));
+      }
+      if (t == 0) {
+        if (a.mean) a.mean[row] = mean;
+        if (a.rstd) a.rstd[row] = rstd;
+      }
+    }
+  }
 }
 
-// One workgroup a row: mean, mean square of the differences, output; the row is read three times (cache hits).
+// Rows too long for the registers of a workgroup: the same sums, the row read three times (twice from the caches).
 template <class T, class P>
-__global__ __launch_bounds__(kThreads) void layer_norm_kernel(hf_layer_norm_args a) {
-  __shared__ float part[kThreads / 64];
-  const int cols = (int)a.cols, tid = (int)threadIdx.x;
+__global__ __launch_bounds__(1024) void layer_norm_long_kernel(hf_layer_norm_args a) {
+  constexpr int VEC = kVec<T>;
+  __shared__ float part[2][16];
+  const int cols = (int)a.cols, tid = (int)threadIdx.x, slots = row_slots<VEC>(cols);
+  auto sum_row = [&](float v, int which) {
+    v = lanes_sum<64>(v);
+    if ((tid & 63) == 0) part[which][tid >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
+    for (int i = 0; i < 16; i++) v += part[which][i];
+    return v;
+  };
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
-    T *y = static_cast<T *>(a.y) + row * a.y_stride;
     float s = 0.0f;
-    for (int c = tid; c < cols; c += kThreads) s += to_f32(x[c]);
-    const float mean = block_sum(s, part) / (float)cols;
-    s = 0.0f;
-    for (int c = tid; c < cols; c += kThreads) {
-      const float d = to_f32(x[c]) - mean;
-      s += d * d;
+    for (int j = tid; j < slots; j += 1024) {
+      const vec_t<T, VEC> v = load_vec<T, VEC>(x + slot_column<VEC>(j, cols));
+      const int skip = slot_repeats<VEC>(j, cols);
+#pragma unroll
+      for (int e = 0; e < VEC; e++) s += e >= skip ? elem<T, VEC>(v, e) : 0.0f;
     }
-    const float rstd = 1.0f / sqrtf(block_sum(s, part) / (float)cols + a.eps);
-    for (int c = tid; c < cols; c += kThreads) {
-      const float w = a.weight ? to_f32(static_cast<const P *>(a.weight)[c]) : 1.0f;
-      const float b = a.bias ? to_f32(static_cast<const P *>(a.bias)[c]) : 0.0f;
-      y[c] = from_f32<T>((to_f32(x[c]) - mean) * rstd * w + b);
+    const float mean = sum_row(s, 0) / (float)cols;
+    s = 0.0f;
+    for (int j = tid; j < slots; j += 1024) {
+      const vec_t<T, VEC> v = load_vec<T, VEC>(x + slot_column<VEC>(j, cols));
+      const int skip = slot_repeats<VEC>(j, cols);
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        const float d = e >= skip ? elem<T, VEC>(v, e) - mean : 0.0f;
+        s += d * d;
+      }
+    }
+    const float rstd = 1.0f / sqrtf(sum_row(s, 1) / (float)cols + a.eps);
+    T *y = static_cast<T *>(a.y) + row * a.y_stride;
+    for (int j = tid; j < slots; j += 1024) {
+      const int c = slot_column<VEC>(j, cols);
+      const vec_t<T, VEC> v = load_vec<T, VEC>(x + c);
+      const vec_t<P, VEC> w = a.weight ? load_vec<P, VEC>(static_cast<const P *>(a.weight) + c) : (vec_t<P, VEC>)(P)1.0f;
+      const vec_t<P, VEC> b = a.bias ? load_vec<P, VEC>(static_cast<const P *>(a.bias) + c) : (vec_t<P, VEC>)(P)0.0f;
+      float out[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; e++) out[e] = (elem<T, VEC>(v, e) - mean) * rstd * elem<P, VEC>(w, e) + elem<P, VEC>(b, e);
+      store_vec<T, VEC>(y + c, round_vec<T, VEC>(out));
     }
     if (tid == 0) {
       if (a.mean) a.mean[row] = mean;
@@ -50,84 +159,47 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(hf_layer_norm_args
   }
 }
 
-template <class T, class P>
-__global__ __launch_bounds__(kThreads) void layer_norm_dx_kernel(hf_layer_norm_backward_args a) {
-  __shared__ float part[kThreads / 64];
-  const int cols = (int)a.cols, tid = (int)threadIdx.x;
-  const P *weight = static_cast<const P *>(a.weight);
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
-    const T *dy = static_cast<const T *>(a.dy) + row * a.dy_stride;
-    T *dx = static_cast<T *>(a.dx) + row * a.dx_stride;
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float sg = 0.0f, sgh = 0.0f;
-    for (int c = tid; c < cols; c += kThreads) {
-      const float g = to_f32(dy[c]) * (weight ? to_f32(weight[c]) : 1.0f);
-      sg += g;
-      sgh += g * ((to_f32(x[c]) - mean) * rstd);
-    }
-    sg = block_sum(sg, part) / (float)cols;
-    sgh = block_sum(sgh, part) / (float)cols;
-    for (int c = tid; c < cols; c += kThreads) {
-      const float g = to_f32(dy[c]) * (weight ? to_f32(weight[c]) : 1.0f);
-      const float h = (to_f32(x[c]) - mean) * rstd;
-      dx[c] = from_f32<T>(rstd * (g - sg - h * sgh));
-    }
-  }
-}
-
-// One thread a column, down all rows.
-template <class T, class P>
-__global__ __launch_bounds__(kThreads) void layer_norm_dparams_kernel(hf_layer_norm_backward_args a) {
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= a.cols) return;
-  const T *x = static_cast<const T *>(a.x) + c, *dy = static_cast<const T *>(a.dy) + c;
-  float dw = 0.0f, db = 0.0f;
-  for (int64_t row = 0; row < a.rows; row++) {
-    const float g = to_f32(dy[row * a.dy_stride]);
-    db += g;
-    if (a.dweight) dw += g * ((to_f32(x[row * a.x_stride]) - a.mean[row]) * a.rstd[row]);
-  }
-  if (a.dweight) static_cast<P *>(a.dweight)[c] = from_f32<P>(dw);
-  if (a.dbias) static_cast<P *>(a.dbias)[c] = from_f32<P>(db);
+// Workgroups a CU: short ones that make a trip or two keep reads and writes of different ones apart in time and are
+// faster than a few that stay (32768 x 8192 bf16: 202, 193, 188, 176 us with 8, 16, 32, 64 a CU).  With float32 weights
+// next to 16-bit rows a workgroup reads as much for its weights as for two rows: half as many (199 -> 187 us).
+template <class T, class P, int VEC, int VPT, int LANES>
+hipError_t norm_rows(const hf_layer_norm_args &a, int cus, hipStream_t s) {
+  constexpr int BLOCK = LANES > 256 ? LANES : 256, GROUPS = BLOCK / LANES;
+  constexpr int kPerCu = (sizeof(P) > sizeof(T) && LANES >= 256 ? 32 : 64) * 256 / BLOCK;
+  const int64_t sets = (a.rows + GROUPS - 1) / GROUPS, most = (int64_t)cus * kPerCu;
+  const int64_t trips = (sets + most - 1) / most;
+  const unsigned grid = (unsigned)((sets + trips - 1) / trips);   // every workgroup makes `trips` trips, or one less
+  hipLaunchKernelGGL((layer_norm_rows_kernel<T, P, VEC, VPT, LANES, BLOCK>), dim3(grid), dim3(BLOCK), 0, s, a, past_caches((size_t)a.rows * (size_t)a.cols * sizeof(T)));
+  return hipGetLastError();
 }
 
 template <class T, class P>
 hipError_t norm_forward(const hf_layer_norm_args &a, int cus, hipStream_t s) {
-  const int64_t grid = std::min<int64_t>(a.rows, (int64_t)cus * 64);
-  hipLaunchKernelGGL((layer_norm_kernel<T, P>), dim3((unsigned)grid), dim3(kThreads), 0, s, a);
-  return hipGetLastError();
-}
-
-template <class T, class P>
-hipError_t norm_backward(const hf_layer_norm_backward_args &a, int cus, hipStream_t s) {
-  if (a.dx && a.rows > 0) {
-    const int64_t grid = std::min<int64_t>(a.rows, (int64_t)cus * 64);
-    hipLaunchKernelGGL((layer_norm_dx_kernel<T, P>), dim3((unsigned)grid), dim3(kThreads), 0, s, a);
-  }
-  if (a.dweight || a.dbias) {
-    const int64_t grid = (a.cols + kThreads - 1) / kThreads;
-    hipLaunchKernelGGL((layer_norm_dparams_kernel<T, P>), dim3((unsigned)grid), dim3(kThreads), 0, s, a);
-  }
+  constexpr int VEC = kVec<T>;
+  if (a.cols < VEC) return norm_rows<T, P, 1, 1, 8>(a, cus, s);
+  const int64_t slots = (a.cols + VEC - 1) / VEC;
+  if (slots <= 8) return norm_rows<T, P, VEC, 1, 8>(a, cus, s);
+  if (slots <= 16) return norm_rows<T, P, VEC, 1, 16>(a, cus, s);
+  if (slots <= 32) return norm_rows<T, P, VEC, 1, 32>(a, cus, s);
+  if (slots <= 64) return norm_rows<T, P, VEC, 1, 64>(a, cus, s);
+  if (slots <= 128) return norm_rows<T, P, VEC, 2, 64>(a, cus, s);
+  if (slots <= 256) return norm_rows<T, P, VEC, 4, 64>(a, cus, s);
+  if (slots <= 512) return norm_rows<T, P, VEC, 4, 128>(a, cus, s);
+  if (slots <= 1024) return norm_rows<T, P, VEC, 4, 256>(a, cus, s);
+  if (slots <= 2048) return norm_rows<T, P, VEC, 2, 1024>(a, cus, s);
+  if (slots <= 4096) return norm_rows<T, P, VEC, 4, 1024>(a, cus, s);
+  const unsigned grid = (unsigned)std::min<int64_t>(a.rows, (int64_t)cus * 2);
+  hipLaunchKernelGGL((layer_norm_long_kernel<T, P>), dim3(grid), dim3(1024), 0, s, a);
   return hipGetLastError();
 }
 
 }  // namespace
-
-size_t layer_norm_backward_workspace(const hf_layer_norm_backward_args &, int) { return 0; }
 
 hipError_t launch_layer_norm(const hf_layer_norm_args &a, int cus, hipStream_t s) {
   if (a.rows == 0) return hipSuccess;
   return with_type(a.type, [&](auto t) {
     using T = decltype(t);
     return a.param_type == HF_F32 ? norm_forward<T, float>(a, cus, s) : norm_forward<T, T>(a, cus, s);
-  });
-}
-
-hipError_t launch_layer_norm_backward(const hf_layer_norm_backward_args &a, int cus, hipStream_t s) {
-  return with_type(a.type, [&](auto t) {
-    using T = decltype(t);
-    return a.param_type == HF_F32 ? norm_backward<T, float>(a, cus, s) : norm_backward<T, T>(a, cus, s);
   });
 }
 

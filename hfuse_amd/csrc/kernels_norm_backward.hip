@@ -1,0 +1,350 @@
+// The gradient of layer norm.
+#include <algorithm>
+
+#include "device/rows.h"
+#include "launch.h"
+
+namespace hfuse {
+namespace {
+
+
+// One pass over the rows: LANES threads hold a row of x and of dy in registers, VPT slots of 16 bytes each, form the two
+// sums over the row that dx needs, write dx, and add dy * h and dy to the 32-bit sums of their columns, which stay in
+// registers for all rows of the workgroup.  The next row is on its way meanwhile.  A workgroup leaves one row of sums for
+// dweight and one for dbias in `parts`; sum_parts_kernel adds them up in the order of the workgroups.
+template <class T, class P, int VEC, int VPT, int LANES, int BLOCK, bool PARAMS>
+__global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_backward_args a, float *parts, bool stream) {
+  constexpr int GROUPS = BLOCK / LANES, WAVES = LANES > 64 ? LANES / 64 : 1;
+  constexpr int SETS = BLOCK / (LANES > 64 ? LANES : 64);   // sets of threads with column sums of their own at the end
+  constexpr bool kKeep = BLOCK < 1024;   // a workgroup of 1024 has 128 registers a thread: weights from the caches, h and g computed twice
+  constexpr bool kAhead = VPT * VEC * BLOCK < 16 * 1024 || BLOCK < 1024;   // ... and a second row of the longest does not fit
+  __shared__ float2 part[2][BLOCK / 64];
+  const int cols = (int)a.cols, t = (int)threadIdx.x % LANES, group = (int)threadIdx.x / LANES;
+  const RowSlots<VEC, VPT, LANES> map(t, cols);
+  const P *weight = static_cast<const P *>(a.weight);
+  const bool want_dx = a.dx != nullptr, want_h = want_dx || a.dweight;   // dbias alone reads dy only
+  auto load_weight = [&](int k) { return weight && want_dx ? load_vec<P, VEC>(weight + map.col[k]) : (vec_t<P, VEC>)(P)1.0f; };
+  vec_t<P, VEC> kept[kKeep ? VPT : 1];
+  if constexpr (kKeep) {
+#pragma unroll
+    for (int k = 0; k < VPT; k++) kept[k] = load_weight(k);
+  }
+  float dw[PARAMS ? VPT : 1][VEC], db[PARAMS ? VPT : 1][VEC];
+#pragma unroll
+  for (int k = 0; k < (PARAMS ? VPT : 1); k++)
+#pragma unroll
+    for (int e = 0; e < VEC; e++) dw[k][e] = db[k][e] = 0.0f;
+
+  const float inv = 1.0f / (float)cols;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  vec_t<T, VEC> next_x[VPT], next_dy[VPT];
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto fetch = [&](int64_t row) {
+    row = min(row, a.rows - 1);
+    const T *dy = static_cast<const T *>(a.dy) + row * a.dy_stride;
+#pragma unroll
+    for (int k = 0; k < VPT; k++) next_dy[k] = stream ? load_vec_stream<T, VEC>(dy + map.col[k]) : load_vec<T, VEC>(dy + map.col[k]);
+    if (want_h) {
+      const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
+#pragma unroll
+      for (int k = 0; k < VPT; k++) next_x[k] = stream ? load_vec_stream<T, VEC>(x + map.col[k]) : load_vec<T, VEC>(x + map.col[k]);
+      next_mean = a.mean[row];
+      next_rstd = a.rstd[row];
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < VPT; k++) next_x[k] = (vec_t<T, VEC>)(T)0.0f;
+  if (kAhead) fetch((int64_t)blockIdx.x * GROUPS + group);
+  int turn = 0;
+  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < a.rows; base += step) {   // all groups of a workgroup make the same trips
+    const int64_t row = base + group;
+    const bool mine = row < a.rows;
+    if (!kAhead) fetch(row);
+    const float mean = next_mean, rstd = next_rstd;
+    vec_t<T, VEC> x[VPT], dy[VPT];
+#pragma unroll
+    for (int k = 0; k < VPT; k++) {
+      x[k] = next_x[k];
+      dy[k] = next_dy[k];
+    }
+    if (kAhead && base + step < a.rows) fetch(row + step);
+    float sg = 0.0f, sgh = 0.0f, hs[kKeep ? VPT : 1][VEC], gs[kKeep ? VPT : 1][VEC];
+    auto h_of = [&](int k, int e) { return (elem<T, VEC>(x[k], e) - mean) * rstd; };
+#pragma unroll
+    for (int k = 0; k < VPT; k++) {
+      const vec_t<P, VEC> w = kKeep ? kept[kKeep ? k : 0] : load_weight(k);
+      auto slot = [&](auto whole) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          const float d = elem<T, VEC>(dy[k], e), h = h_of(k, e), g = d * elem<P, VEC>(w, e);
+          if constexpr (kKeep) {
+            hs[k][e] = h;
+            gs[k][e] = g;
+          }
+          if (whole() || e >= map.skip[k]) {
+            sg += g;
+            sgh += g * h;
+          }
+          if (PARAMS && mine) {   // (repeated columns are summed twice, alike)
+            dw[k][e] += d * h;
+            db[k][e] += d;
+          }
+        }
+      };
+      if (map.whole[k]) slot([] { return true; });
+      else slot([] { return false; });
+    }
+    if (!want_dx) continue;
+    sg = lanes_sum<(LANES < 64 ? LANES : 64)>(sg);
+    sgh = lanes_sum<(LANES < 64 ? LANES : 64)>(sgh);
+    if constexpr (LANES > 64) {
+      if ((threadIdx.x & 63u) == 0) part[turn][threadIdx.x >> 6] = make_float2(sg, sgh);
+      __syncthreads();   // two slots in turn: a slot is written again only behind the other one's barrier
+      sg = sgh = 0.0f;
+#pragma unroll
+      for (int i = 0; i < WAVES; i++) {
+        const float2 v = part[turn][group * WAVES + i];
+        sg += v.x;
+        sgh += v.y;
+      }
+      turn ^= 1;
+    }
+    sg *= inv * rstd;
+    sgh *= inv * rstd;
+    if (mine) {
+      T *dx = static_cast<T *>(a.dx) + row * a.dx_stride;
+#pragma unroll
+      for (int k = 0; k < VPT; k++) {
+        if (map.skip[k] == VEC) continue;
+        float out[VEC];
+        if constexpr (kKeep) {
+#pragma unroll
+          for (int e = 0; e < VEC; e++) out[e] = gs[k][e] * rstd - (sg + hs[k][e] * sgh);
+        } else {
+          const vec_t<P, VEC> w = load_weight(k);
+#pragma unroll
+          for (int e = 0; e < VEC; e++) out[e] = elem<T, VEC>(dy[k], e) * elem<P, VEC>(w, e) * rstd - (sg + h_of(k, e) * sgh);
+        }
+        store_vec_stream<T, VEC>(dx + map.col[k], round_vec<T, VEC>(out));
+      }
+    }
+  }
+
+  if constexpr (PARAMS) {
+    const size_t width = (size_t)row_slots<VEC>(cols) * VEC;
+    float *dw_part = parts + (size_t)blockIdx.x * 2 * width, *db_part = dw_part + width;
+    constexpr int SPAN = LANES > 64 ? LANES : 64;   // threads of a set
+    __shared__ float sums[SETS > 1 ? (SETS - 1) * SPAN * VEC : 1];
+    const int set = (int)threadIdx.x / SPAN, in_set = (int)threadIdx.x % SPAN;
+#pragma unroll
+    for (int k = 0; k < VPT; k++) {
+#pragma unroll
+      for (int which = 0; which < 2; which++) {
+        float v[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          v[e] = which ? db[k][e] : dw[k][e];
+#pragma unroll
+          for (int m = LANES; m < 64; m <<= 1) v[e] += __shfl_xor(v[e], m);   // the groups inside a wave
+        }
+        if constexpr (SETS > 1) {
+          if (set > 0)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) sums[((set - 1) * VEC + e) * SPAN + in_set] = v[e];
+          __syncthreads();
+          if (set == 0)
+            for (int i = 0; i < SETS - 1; i++)
+#pragma unroll
+              for (int e = 0; e < VEC; e++) v[e] += sums[(i * VEC + e) * SPAN + in_set];
+          __syncthreads();
+        }
+        if (set == 0 && in_set < LANES && map.skip[k] != VEC)
+          store_vec<float, VEC>((which ? db_part : dw_part) + (size_t)(t + k * LANES) * VEC, round_vec<float, VEC>(v));
+      }
+    }
+  }
+}
+
+// Rows too long for the registers of a workgroup: dx by itself, the rows read twice (the second time from the caches) ...
+template <class T, class P>
+__global__ __launch_bounds__(1024) void layer_norm_long_dx_kernel(hf_layer_norm_backward_args a) {
+  constexpr int VEC = kVec<T>;
+  __shared__ float2 part[2][16];
+  const int cols = (int)a.cols, tid = (int)threadIdx.x, slots = row_slots<VEC>(cols);
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const T *x = static_cast<const T *>(a.x) + row * a.x_stride, *dy = static_cast<const T *>(a.dy) + row * a.dy_stride;
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float sg = 0.0f, sgh = 0.0f;
+    auto weights = [&](int c) { return a.weight ? load_vec<P, VEC>(static_cast<const P *>(a.weight) + c) : (vec_t<P, VEC>)(P)1.0f; };
+    for (int j = tid; j < slots; j += 1024) {
+      const int c = slot_column<VEC>(j, cols), skip = slot_repeats<VEC>(j, cols);
+      const vec_t<T, VEC> xv = load_vec<T, VEC>(x + c), dv = load_vec<T, VEC>(dy + c);
+      const vec_t<P, VEC> wv = weights(c);
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        const float g = elem<T, VEC>(dv, e) * elem<P, VEC>(wv, e);
+        if (e >= skip) {
+          sg += g;
+          sgh += g * ((elem<T, VEC>(xv, e) - mean) * rstd);
+        }
+      }
+    }
+    sg = lanes_sum<64>(sg);
+    sgh = lanes_sum<64>(sgh);
+    if ((tid & 63) == 0) part[turn][tid >> 6] = make_float2(sg, sgh);
+    __syncthreads();
+    sg = sgh = 0.0f;
+    for (int i = 0; i < 16; i++) {
+      sg += part[turn][i].x;
+      sgh += part[turn][i].y;
+    }
+    sg /= (float)cols;
+    sgh /= (float)cols;
+    T *dx = static_cast<T *>(a.dx) + row * a.dx_stride;
+    for (int j = tid; j < slots; j += 1024) {
+      const int c = slot_column<VEC>(j, cols);
+      const vec_t<T, VEC> xv = load_vec<T, VEC>(x + c), dv = load_vec<T, VEC>(dy + c);
+      const vec_t<P, VEC> wv = weights(c);
+      float out[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; e++)
+        out[e] = rstd * (elem<T, VEC>(dv, e) * elem<P, VEC>(wv, e) - sg - (elem<T, VEC>(xv, e) - mean) * rstd * sgh);
+      store_vec<T, VEC>(dx + c, round_vec<T, VEC>(out));
+    }
+  }
+}
+
+// ... and the sums down the columns, a thread a column over every gridDim.y-th row.
+template <class T>
+__global__ __launch_bounds__(256) void layer_norm_long_params_kernel(hf_layer_norm_backward_args a, float *parts) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.cols) return;
+  float dw = 0.0f, db = 0.0f;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const float d = to_f32(static_cast<const T *>(a.dy)[row * a.dy_stride + c]);
+    if (a.dweight) dw += d * ((to_f32(static_cast<const T *>(a.x)[row * a.x_stride + c]) - a.mean[row]) * a.rstd[row]);
+    db += d;
+  }
+  float *part = parts + (size_t)blockIdx.y * 2 * (size_t)a.cols + c;
+  part[0] = dw;
+  part[a.cols] = db;
+}
+
+// dweight and dbias from `nparts` rows of sums each: 64 columns a workgroup, whose sixteen waves take the rows in turn;
+// their sums are added in the order of the waves.  Column c of the parts is slot c / vec, element c % vec.
+template <class P>
+__global__ __launch_bounds__(1024) void sum_parts_kernel(const float *parts, int nparts, int vec, int cols, P *dweight, P *dbias) {
+  __shared__ float sums[16][64];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const int width = (int)(((unsigned)cols + (unsigned)vec - 1) / (unsigned)vec) * vec;
+  const int at = (int)blockIdx.x * 64 + lane;
+  P *out = blockIdx.y ? dbias : dweight;
+  if (!out) return;
+  const float *p = parts + (size_t)blockIdx.y * width + min(at, width - 1);
+  float s = 0.0f;
+#pragma unroll 8
+  for (int i = wave; i < nparts; i += 16) s += p[(size_t)i * 2 * (size_t)width];
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && at < width) {
+    s = 0.0f;
+    for (int i = 0; i < 16; i++) s += sums[i][lane];
+    out[min(at / vec * vec, cols - vec) + at % vec] = from_f32<P>(s);
+  }
+}
+
+// How the gradient is cut: threads to a row, slots to a thread, workgroups.
+struct GradPlan {
+  int vec, vpt, lanes, block;
+  bool in_registers;
+  unsigned grid;   // workgroups with a part of the columns' sums each
+  size_t bytes;
+};
+
+GradPlan plan_grad(const hf_layer_norm_backward_args &a, int cus) {
+  GradPlan p;
+  const int full = a.type == HF_F32 ? kVec<float> : kVec<bf16_t>;
+  p.vec = a.cols < full ? 1 : full;
+  const int64_t slots = (a.cols + p.vec - 1) / p.vec;
+  p.vpt = slots <= 64 ? 1 : a.type == HF_F32 && slots > 2048 ? 4 : 2;
+  p.lanes = 8;
+  while (p.lanes < 1024 && (int64_t)p.lanes * p.vpt < slots) p.lanes *= 2;
+  p.in_registers = (int64_t)p.lanes * p.vpt >= slots;
+  p.block = p.lanes > 512 ? 1024 : 512;
+  if (p.in_registers) {
+    const int64_t groups = p.block / p.lanes, sets = (a.rows + groups - 1) / groups, most = (int64_t)cus;
+    const int64_t trips = std::max<int64_t>(1, (sets + most - 1) / most);
+    p.grid = (unsigned)((sets + trips - 1) / trips);   // every workgroup makes `trips` trips, or one less
+  } else {
+    p.vec = 1;
+    p.grid = (unsigned)std::min<int64_t>(a.rows, 64);
+  }
+  const size_t width = (size_t)((a.cols + p.vec - 1) / p.vec) * p.vec;
+  p.bytes = a.dweight || a.dbias ? (size_t)p.grid * 2 * width * sizeof(float) : 0;
+  return p;
+}
+
+template <class T, class P, int VEC, int VPT, int LANES>
+hipError_t grad_rows(const hf_layer_norm_backward_args &a, const GradPlan &p, hipStream_t s) {
+  constexpr int BLOCK = LANES > 512 ? 1024 : 512;
+  const bool stream = past_caches((size_t)a.rows * (size_t)a.cols * sizeof(T) * 2);
+  if (a.dweight || a.dbias)
+    hipLaunchKernelGGL((layer_norm_grad_kernel<T, P, VEC, VPT, LANES, BLOCK, true>), dim3(p.grid), dim3(BLOCK), 0, s, a, static_cast<float *>(a.workspace), stream);
+  else
+    hipLaunchKernelGGL((layer_norm_grad_kernel<T, P, VEC, VPT, LANES, BLOCK, false>), dim3(p.grid), dim3(BLOCK), 0, s, a, nullptr, stream);
+  return hipGetLastError();
+}
+
+template <class T, class P>
+hipError_t grad_in_registers(const hf_layer_norm_backward_args &a, const GradPlan &p, hipStream_t s) {
+  constexpr int VEC = kVec<T>;
+  if (p.vec == 1) return grad_rows<T, P, 1, 1, 8>(a, p, s);
+  if (p.vpt == 1) {
+    if (p.lanes == 8) return grad_rows<T, P, VEC, 1, 8>(a, p, s);
+    if (p.lanes == 16) return grad_rows<T, P, VEC, 1, 16>(a, p, s);
+    if (p.lanes == 32) return grad_rows<T, P, VEC, 1, 32>(a, p, s);
+    return grad_rows<T, P, VEC, 1, 64>(a, p, s);
+  }
+  if constexpr (VEC == 4) {
+    if (p.vpt == 4) return grad_rows<T, P, VEC, 4, 1024>(a, p, s);
+  }
+  if (p.lanes == 64) return grad_rows<T, P, VEC, 2, 64>(a, p, s);
+  if (p.lanes == 128) return grad_rows<T, P, VEC, 2, 128>(a, p, s);
+  if (p.lanes == 256) return grad_rows<T, P, VEC, 2, 256>(a, p, s);
+  if (p.lanes == 512) return grad_rows<T, P, VEC, 2, 512>(a, p, s);
+  return grad_rows<T, P, VEC, 2, 1024>(a, p, s);
+}
+
+template <class T, class P>
+hipError_t norm_backward(const hf_layer_norm_backward_args &a, int cus, hipStream_t s) {
+  const GradPlan p = plan_grad(a, cus);
+  const bool params = a.dweight || a.dbias;
+  float *parts = static_cast<float *>(a.workspace);
+  if (a.rows > 0 && p.in_registers) {
+    const hipError_t e = grad_in_registers<T, P>(a, p, s);
+    if (e != hipSuccess) return e;
+  } else if (a.rows > 0) {
+    if (a.dx) hipLaunchKernelGGL((layer_norm_long_dx_kernel<T, P>), dim3((unsigned)std::min<int64_t>(a.rows, (int64_t)cus * 2)), dim3(1024), 0, s, a);
+    if (params) hipLaunchKernelGGL((layer_norm_long_params_kernel<T>), dim3((unsigned)((a.cols + 255) / 256), p.grid), dim3(256), 0, s, a, parts);
+  }
+  if (params) {
+    const int64_t width = (a.cols + p.vec - 1) / p.vec * p.vec;
+    hipLaunchKernelGGL((sum_parts_kernel<P>), dim3((unsigned)((width + 63) / 64), 2), dim3(1024), 0, s, parts, (int)(a.rows > 0 ? p.grid : 0), p.vec,
+                       (int)a.cols, static_cast<P *>(a.dweight), static_cast<P *>(a.dbias));
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+size_t layer_norm_backward_workspace(const hf_layer_norm_backward_args &a, int cus) { return plan_grad(a, cus).bytes; }
+
+hipError_t launch_layer_norm_backward(const hf_layer_norm_backward_args &a, int cus, hipStream_t s) {
+  return with_type(a.type, [&](auto t) {
+    using T = decltype(t);
+    return a.param_type == HF_F32 ? norm_backward<T, float>(a, cus, s) : norm_backward<T, T>(a, cus, s);
+  });
+}
+
+}  // namespace hfuse
