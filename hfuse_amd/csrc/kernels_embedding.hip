@@ -7,18 +7,35 @@
 namespace hfuse {
 namespace {
 
-constexpr int kThreads = 256;
-
-// One workgroup a token.
-template <class T, class I>
-__global__ __launch_bounds__(kThreads) void embedding_kernel(hf_embedding_args a) {
-  for (int64_t i = blockIdx.x; i < a.ntokens; i += gridDim.x) {
-    const int64_t t = (int64_t) static_cast<const I *>(a.tokens)[i];
-    T *out = static_cast<T *>(a.out) + i * a.out_stride;
-    const bool used = t >= 0 && t < a.vocab;
-    const T *w = static_cast<const T *>(a.weight) + (used ? t : 0) * a.weight_stride;
-    for (int64_t c = threadIdx.x; c < a.cols; c += kThreads)
-      out[c] = used ? (a.scale == 1.0f ? w[c] : from_f32<T>(to_f32(w[c]) * a.scale)) : from_f32<T>(0.0f);
+// A group of `lanes` lanes copies U of its slots of a row at once: all its reads are on their way before the first store.
+template <class T, class I, int VEC, int U>
+__global__ __launch_bounds__(256) void embedding_kernel(hf_embedding_args a, int lanes_log2, unsigned tiles) {
+  const unsigned lanes = 1u << lanes_log2, lane = threadIdx.x & (lanes - 1);
+  const unsigned long long group = ((unsigned long long)blockIdx.x * 256u + threadIdx.x) >> lanes_log2;
+  const int64_t i = (int64_t)(group / tiles);
+  const int tile = (int)(group % tiles);
+  if (i >= a.ntokens) return;
+  const int64_t t = (int64_t) static_cast<const I *>(a.tokens)[i];
+  const bool used = t >= 0 && t < a.vocab;
+  const T *w = static_cast<const T *>(a.weight) + (used ? t : 0) * a.weight_stride;
+  T *out = static_cast<T *>(a.out) + i * a.out_stride;
+  const int cols = (int)a.cols, slots = row_slots<VEC>(cols);
+  int col[U];
+  vec_t<T, VEC> v[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    col[u] = slot_column<VEC>(min((tile * U + u) * (int)lanes + (int)lane, slots - 1), cols);   // (lanes behind the row repeat its last slot)
+    v[u] = used ? load_vec<T, VEC>(w + col[u]) : (vec_t<T, VEC>)(T)0.0f;
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    if (a.scale != 1.0f) {   // (1: the table's bits)
+      float f[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; e++) f[e] = elem<T, VEC>(v[u], e) * a.scale;
+      v[u] = round_vec<T, VEC>(f);
+    }
+    if ((tile * U + u) * (int)lanes + (int)lane < slots) store_vec_stream<T, VEC>(out + col[u], v[u]);
   }
 }
 
@@ -58,6 +75,18 @@ struct ZeroRows {
   unsigned element;   // bytes of an element
 };
 
+__device__ __forceinline__ void zero_row(const hf_embedding_backward_args &a, const ZeroRows &z, size_t v, unsigned lane) {
+  const unsigned lanes = 1u << z.lanes_log2, bytes = (unsigned)a.cols * z.element;
+  unsigned char *row = static_cast<unsigned char *>(a.dweight) + v * (size_t)a.dweight_stride * z.element;
+  typedef unsigned short word_t;   // rows are aligned to an element, of two bytes or more
+  if (bytes >= 16) {
+    for (unsigned j = lane * 16u; j < bytes; j += lanes * 16u)
+      store_vec_stream<word_t, 8>(reinterpret_cast<word_t *>(row + min(j, bytes - 16u)), (vec_t<word_t, 8>)(word_t)0);
+  } else {
+    for (unsigned j = lane * 2u; j < bytes; j += lanes * 2u) *reinterpret_cast<word_t *>(row + j) = 0;
+  }
+}
+
 template <class I>
 __device__ __forceinline__ void write_zero_rows(const hf_embedding_backward_args &a, const unsigned *owner, const ZeroRows &z, unsigned block) {
   const size_t at = (size_t)block * 256u + threadIdx.x;
@@ -67,16 +96,7 @@ __device__ __forceinline__ void write_zero_rows(const hf_embedding_backward_args
   // `owner` was never cleared: what it says is a claim, true if the position it gives names this token
   const unsigned i = owner[v];
   if (i < (unsigned)a.ntokens && (int64_t) static_cast<const I *>(a.tokens)[i] == (int64_t)v && (int64_t)v != a.padding_idx) return;
-  const unsigned lanes = 1u << z.lanes_log2, lane = (unsigned)at & (lanes - 1);
-  const unsigned bytes = (unsigned)a.cols * z.element;
-  unsigned char *row = static_cast<unsigned char *>(a.dweight) + v * (size_t)a.dweight_stride * z.element;
-  typedef unsigned short word_t;   // rows are aligned to an element, of two bytes or more
-  if (bytes >= 16) {
-    for (unsigned j = lane * 16u; j < bytes; j += lanes * 16u)
-      store_vec_stream<word_t, 8>(reinterpret_cast<word_t *>(row + min(j, bytes - 16u)), (vec_t<word_t, 8>)(word_t)0);
-  } else {
-    for (unsigned j = lane * 2u; j < bytes; j += lanes * 2u) *reinterpret_cast<word_t *>(row + j) = 0;
-  }
+  zero_row(a, z, v, (unsigned)at & ((1u << z.lanes_log2) - 1u));
 }
 
 // Entry i of the list in hand: of the tokens themselves for the first digit ({i, ~0} for one outside the table or equal to
@@ -98,6 +118,43 @@ __device__ __forceinline__ uint2 list_entry(const hf_embedding_backward_args &a,
     const bool used = hi == 0 && lo < (unsigned)a.vocab && (a.padding_idx < 0 || lo != (unsigned)a.padding_idx);
     return make_uint2(i, used ? lo : ~0u);
   }
+}
+
+// Numbers the equal digits of a wave's 64 entries in the order of the lanes, behind the ones the wave has counted before.
+// The lanes with the same digit are found with one ballot a bit.
+__device__ __forceinline__ unsigned rank_equal(unsigned digit, bool used, int bits, unsigned lane, unsigned *count) {
+  unsigned long long same = __ballot(used);
+  for (int b = 0; b < bits; b++) {
+    const bool one = (digit >> b) & 1u;
+    const unsigned long long ones = __ballot(one);
+    same &= one ? ones : ~ones;
+  }
+  unsigned rank = 0;
+  if (used) {
+    const int leader = __builtin_ctzll(same);
+    if ((int)lane == leader) rank = atomicAdd(&count[digit], (unsigned)__builtin_popcountll(same));
+    rank = (unsigned)__shfl((int)rank, leader) + (unsigned)__builtin_popcountll(same & ((1ull << lane) - 1ull));
+  }
+  return rank;
+}
+
+// Inclusive sum over the threads of a workgroup in their order, and the sum of all; one barrier.
+__device__ __forceinline__ unsigned scan_block(unsigned v, unsigned *part, unsigned &all) {
+  const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const unsigned u = __shfl_up(v, m);
+    if (lane >= (unsigned)m) v += u;
+  }
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  all = 0;
+#pragma unroll
+  for (unsigned w = 0; w < kSortWaves; w++) {
+    if (w < wave) v += part[w];
+    all += part[w];
+  }
+  return v;
 }
 
 // Workgroups [0, tiles): how often each value of the digit occurs in a tile; the first digit's launch notes an owner of
@@ -163,20 +220,8 @@ __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(hf_embedding
       total[1] += c.y;
     }
   }
-  unsigned upto = total[0] + total[1];
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const unsigned v = __shfl_up(upto, m);
-    if (lane >= (unsigned)m) upto += v;
-  }
-  if (lane == 63) scan[wave] = upto;
-  __syncthreads();
-  unsigned all = 0;
-#pragma unroll
-  for (unsigned w = 0; w < kSortWaves; w++) {
-    if (w < wave) upto += scan[w];
-    all += scan[w];
-  }
+  unsigned all;
+  const unsigned upto = scan_block(total[0] + total[1], scan, all);
   if (tid * kOwn < buckets) {
     base[tid * kOwn] = upto - total[0] - total[1] + before[0];
     base[tid * kOwn + 1] = upto - total[1] + before[1];
@@ -192,22 +237,8 @@ __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(hf_embedding
     for (unsigned b = lane; b < buckets; b += 64) count[wave][b] = 0;   // a wave's counters are its own
     unsigned rank[kSortKeys];
 #pragma unroll
-    for (int u = 0; u < kSortKeys; u++) {
-      const unsigned d = (entry[u].y >> shift) & (buckets - 1);
-      const bool used = entry[u].y != ~0u;
-      unsigned long long same = __ballot(used);
-      for (int b = 0; b < bits; b++) {
-        const bool one = (d >> b) & 1u;
-        const unsigned long long ones = __ballot(one);
-        same &= one ? ones : ~ones;
-      }
-      rank[u] = 0;
-      if (used) {
-        const int leader = __builtin_ctzll(same);
-        if ((int)lane == leader) rank[u] = atomicAdd(&count[wave][d], (unsigned)__builtin_popcountll(same));
-        rank[u] = (unsigned)__shfl((int)rank[u], leader) + (unsigned)__builtin_popcountll(same & ((1ull << lane) - 1ull));
-      }
-    }
+    for (int u = 0; u < kSortKeys; u++)
+      rank[u] = rank_equal((entry[u].y >> shift) & (buckets - 1), entry[u].y != ~0u, bits, lane, count[wave]);
     __syncthreads();
     for (unsigned b = tid; b < buckets; b += kSortThreads) {   // counts -> first places; the tile's next step follows
       unsigned at = base[b];
@@ -224,6 +255,78 @@ __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(hf_embedding
     for (int u = 0; u < kSortKeys; u++)
       if (entry[u].y != ~0u) out[count[wave][(entry[u].y >> shift) & (buckets - 1)] + rank[u]] = entry[u];
     __syncthreads();   // (a faster wave clears its own counters only, but `base` and the places above are everyone's)
+  }
+}
+
+// Few tokens (kSortStep at most), one launch: workgroup 0 sorts them in its LDS, digit by digit; the others have `rows` rows
+// of the table each, look through the tokens themselves and write the rows of zeros.
+constexpr unsigned kFewRows = 256;   // rows of a workgroup at most
+template <class I>
+__global__ __launch_bounds__(kSortThreads) void sort_few_kernel(hf_embedding_backward_args a, TableScratch sc, int passes, int bits, unsigned rows,
+                                                                ZeroRows z) {
+  __shared__ uint2 list[kSortStep];
+  __shared__ unsigned count[kSortWaves][kMaxBuckets], scan[kSortWaves];
+  const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  uint2 entry[kSortKeys];
+#pragma unroll
+  for (int u = 0; u < kSortKeys; u++) entry[u] = list_entry<I, true>(a, nullptr, (wave * kSortKeys + u) * 64u + lane, (unsigned)a.ntokens);
+  if (blockIdx.x > 0) {
+    unsigned *present = count[0];
+    const size_t first = (size_t)(blockIdx.x - 1) * rows;
+    const unsigned mine = (unsigned)min((size_t)rows, (size_t)a.vocab - first);
+    if (tid < kFewRows) present[tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kSortKeys; u++) {
+      const size_t r = (size_t)entry[u].y - first;
+      if (entry[u].y != ~0u && r < mine) present[r] = 1;
+    }
+    __syncthreads();
+    for (unsigned r = tid >> z.lanes_log2; r < mine; r += kSortThreads >> z.lanes_log2)
+      if (!present[r]) zero_row(a, z, first + r, tid & ((1u << z.lanes_log2) - 1u));
+    return;
+  }
+  const unsigned buckets = 1u << bits;
+  unsigned used = 0;
+  for (int pass = 0; pass < passes; pass++) {
+    const int shift = pass * bits;
+    for (unsigned b = lane; b < buckets; b += 64) count[wave][b] = 0;   // a wave's counters are its own
+    unsigned rank[kSortKeys];
+#pragma unroll
+    for (int u = 0; u < kSortKeys; u++)
+      rank[u] = rank_equal((entry[u].y >> shift) & (buckets - 1), entry[u].y != ~0u, bits, lane, count[wave]);
+    __syncthreads();
+    constexpr int kOwn = kMaxBuckets / kSortThreads;
+    unsigned total = 0;
+    if (tid * kOwn < buckets)
+      for (int o = 0; o < kOwn; o++)
+        for (int w = 0; w < kSortWaves; w++) total += count[w][tid * kOwn + o];
+    unsigned at = scan_block(total, scan, used) - total;
+    if (tid * kOwn < buckets)
+      for (int o = 0; o < kOwn; o++)
+        for (int w = 0; w < kSortWaves; w++) {
+          const unsigned c = count[w][tid * kOwn + o];
+          count[w][tid * kOwn + o] = at;
+          at += c;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kSortKeys; u++)
+      if (entry[u].y != ~0u) list[count[wave][(entry[u].y >> shift) & (buckets - 1)] + rank[u]] = entry[u];
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kSortKeys; u++) {
+      const unsigned i = (wave * kSortKeys + u) * 64u + lane;
+      entry[u] = i < used ? list[i] : make_uint2(0, ~0u);
+    }
+    __syncthreads();   // the list and the counters are written again
+  }
+#pragma unroll
+  for (int u = 0; u < kSortKeys; u++)
+    if (entry[u].y != ~0u) sc.order[(wave * kSortKeys + u) * 64u + lane] = entry[u];
+  if (tid == 0) {
+    sc.state[0] = used;
+    sc.state[1] = 0;
   }
 }
 
@@ -387,6 +490,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(hf_embedding
 
 constexpr int kMaxChunk = 64, kSumWaves = 16;   // entries of a chunk at most; waves a CU should have at least
 
+constexpr int64_t kFewBytes = 8192;   // bytes of the table to a workgroup of sort_few_kernel
+
 // How the launches are cut: columns into slots and tiles, sorted entries into chunks, the token's bits into digits.
 struct TablePlan {
   int vec, lanes_log2, slots, passes, digit_bits, zero_log2;
@@ -454,6 +559,13 @@ hipError_t sum_tokens(const hf_embedding_backward_args &a, const TablePlan &p, c
 
 template <class I>
 hipError_t sort_tokens(const hf_embedding_backward_args &a, const TablePlan &p, const TableScratch &sc, const ZeroRows &all, hipStream_t s) {
+  if (a.ntokens <= kSortStep) {
+    const int64_t row_bytes = a.cols * (int64_t)all.element;
+    int64_t rows = std::max<int64_t>(1, std::min<int64_t>(kFewRows, kFewBytes / row_bytes));
+    const unsigned blocks = (unsigned)((a.vocab + rows - 1) / rows);
+    hipLaunchKernelGGL((sort_few_kernel<I>), dim3(1 + blocks), dim3(kSortThreads), 0, s, a, sc, p.passes, p.digit_bits, (unsigned)rows, all);
+    return hipGetLastError();
+  }
   // the rows of zeros are shared evenly among the launches behind the first, which finds out what they are
   const unsigned parts = 2u * (unsigned)p.passes - 1u;
   ZeroRows z = {0, 0, all.lanes_log2, all.element};
@@ -515,14 +627,34 @@ hipError_t embed_backward(const hf_embedding_backward_args &a, int cus, hipStrea
 
 size_t embedding_backward_workspace(const hf_embedding_backward_args &a, int cus) { return plan_table(a, cus).bytes; }
 
+namespace {
+template <class T, class I, int VEC, int U>
+hipError_t look_up(const hf_embedding_args &a, int lanes_log2, hipStream_t s) {
+  const int64_t slots = (a.cols + VEC - 1) / VEC, per_tile = (int64_t)U << lanes_log2, tiles = (slots + per_tile - 1) / per_tile;
+  const int64_t blocks = (((a.ntokens * tiles) << lanes_log2) + 255) / 256;
+  hipLaunchKernelGGL((embedding_kernel<T, I, VEC, U>), dim3((unsigned)blocks), dim3(256), 0, s, a, lanes_log2, (unsigned)tiles);
+  return hipGetLastError();
+}
+
+template <class T, class I>
+hipError_t embed_forward(const hf_embedding_args &a, int cus, hipStream_t s) {
+  constexpr int VEC = kVec<T>;
+  const bool narrow = a.cols < VEC;
+  const int64_t slots = narrow ? a.cols : (a.cols + VEC - 1) / VEC;
+  int lanes_log2 = 6;
+  while (lanes_log2 > 0 && (1 << (lanes_log2 - 1)) >= slots) lanes_log2--;
+  if (narrow) return look_up<T, I, 1, 1>(a, lanes_log2, s);
+  const int64_t waves = (a.ntokens * slots) >> 6;   // with one slot a lane
+  if (slots > 64 && waves > (int64_t)cus * 32) return look_up<T, I, VEC, 2>(a, lanes_log2, s);
+  return look_up<T, I, VEC, 1>(a, lanes_log2, s);
+}
+}  // namespace
+
 hipError_t launch_embedding(const hf_embedding_args &a, int cus, hipStream_t s) {
   if (a.ntokens == 0) return hipSuccess;
-  const unsigned grid = (unsigned)std::min<int64_t>(a.ntokens, (int64_t)cus * 64);
   return with_type(a.type, [&](auto t) {
     using T = decltype(t);
-    if (a.index_type == HF_I64) hipLaunchKernelGGL((embedding_kernel<T, int64_t>), dim3(grid), dim3(kThreads), 0, s, a);
-    else hipLaunchKernelGGL((embedding_kernel<T, int32_t>), dim3(grid), dim3(kThreads), 0, s, a);
-    return hipGetLastError();
+    return a.index_type == HF_I64 ? embed_forward<T, int64_t>(a, cus, s) : embed_forward<T, int32_t>(a, cus, s);
   });
 }
 

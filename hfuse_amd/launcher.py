@@ -375,15 +375,15 @@ def histc_args(x, out, nbins, lo, hi) -> L.HistcArgs:
 
 
 # ------------------------------------------------------------ token-model operators
-def element_type(t) -> int:
-    """HF_F32 / HF_BF16 / HF_F16 of a tensor or dtype."""
-    import torch
-    return {torch.float32: L.HF_F32, torch.bfloat16: L.HF_BF16, torch.float16: L.HF_F16}[getattr(t, "dtype", t)]
+_TYPE_CODES: dict = {}   # torch dtype -> HF_F32 / HF_BF16 / HF_F16, HF_I32 / HF_I64 (filled on first use: torch is imported late)
 
 
-def index_type(t) -> int:
-    import torch
-    return {torch.int32: L.HF_I32, torch.int64: L.HF_I64}[t.dtype]
+def _code(t) -> int:
+    if not _TYPE_CODES:
+        import torch
+        _TYPE_CODES.update({torch.float32: L.HF_F32, torch.bfloat16: L.HF_BF16, torch.float16: L.HF_F16,
+                            torch.int32: L.HF_I32, torch.int64: L.HF_I64})
+    return _TYPE_CODES[t.dtype]
 
 
 def _ptr(t):
@@ -391,44 +391,43 @@ def _ptr(t):
 
 
 def _row_stride(t, cols: int) -> int:
-    """Elements between the rows of a [..., cols] tensor whose leading dimensions step evenly (any value for one row)."""
-    return t.stride(-2) if t.dim() == 2 and t.shape[0] > 1 else cols
+    """Elements between the rows of `cols` elements of a contiguous tensor, or of a [rows, cols] one with dense rows."""
+    return cols if t is None or t.is_contiguous() else t.stride(0)
 
 
-def layer_norm_args(x, y, weight=None, bias=None, mean=None, rstd=None, eps: float = 1e-5) -> L.LayerNormArgs:
-    """x, y: [rows, cols], their rows dense; weight / bias: [cols]; mean / rstd: [rows] float32."""
-    rows, cols = x.shape
-    param = weight if weight is not None else bias
-    return L.LayerNormArgs(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean), _ptr(rstd), rows, cols,
-                           _row_stride(x, cols), _row_stride(y, cols), eps, element_type(x),
-                           element_type(x if param is None else param))
+def layer_norm_args(x, y, weight=None, bias=None, mean=None, rstd=None, eps: float = 1e-5, cols: int = 0) -> L.LayerNormArgs:
+    """x, y: contiguous, or [rows, cols] with dense rows; cols: 0 = x's last dimension; mean / rstd: [rows] float32."""
+    cols = cols or x.shape[-1]
+    param = weight if weight is not None else bias if bias is not None else x
+    return L.LayerNormArgs(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean), _ptr(rstd), x.numel() // cols, cols,
+                           _row_stride(x, cols), _row_stride(y, cols), eps, _code(x), _code(param))
 
 
-def layer_norm_backward_args(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=None,
-                             workspace=None) -> L.LayerNormBackwardArgs:
-    """dy, x, dx: [rows, cols]; dweight / dbias: [cols] of the parameters' type; workspace: a byte tensor of workspace_bytes()."""
-    rows, cols = x.shape
-    param = next((t for t in (weight, dweight, dbias) if t is not None), x)
+def layer_norm_backward_args(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=None, workspace=None,
+                             cols: int = 0) -> L.LayerNormBackwardArgs:
+    """dy, x, dx as x of layer_norm_args; dweight / dbias: [cols] of one type; workspace: a byte tensor of workspace_bytes()."""
+    cols = cols or x.shape[-1]
+    param = weight if weight is not None else dweight if dweight is not None else dbias if dbias is not None else x
     return L.LayerNormBackwardArgs(_ptr(dy), _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight), _ptr(dbias),
-                                   rows, cols, _row_stride(dy, cols), _row_stride(x, cols),
-                                   cols if dx is None else _row_stride(dx, cols), element_type(x), element_type(param),
-                                   _ptr(workspace), 0 if workspace is None else workspace.numel())
+                                   x.numel() // cols, cols, _row_stride(dy, cols), _row_stride(x, cols), _row_stride(dx, cols),
+                                   _code(x), _code(param), _ptr(workspace), 0 if workspace is None else workspace.numel())
 
 
 def embedding_args(tokens, weight, out, scale: float = 1.0) -> L.EmbeddingArgs:
-    """tokens: int32 / int64, contiguous; weight: [vocab, cols]; out: [tokens, cols]."""
+    """tokens: int32 / int64, contiguous; weight: [vocab, cols], rows dense; out: contiguous, or [tokens, cols] with dense rows."""
     vocab, cols = weight.shape
     return L.EmbeddingArgs(_ptr(tokens), _ptr(weight), _ptr(out), tokens.numel(), vocab, cols, _row_stride(weight, cols),
-                           _row_stride(out, cols), scale, element_type(weight), index_type(tokens))
+                           _row_stride(out, cols), scale, _code(weight), _code(tokens))
 
 
 def embedding_backward_args(dy, tokens, dweight, scale: float = 1.0, padding_idx: int = -1,
                             workspace=None) -> L.EmbeddingBackwardArgs:
-    """dy: [tokens, cols]; dweight: [vocab, cols]; padding_idx < 0: none; workspace: a byte tensor of workspace_bytes()."""
+    """dy: contiguous, or [tokens, cols] with dense rows; dweight: [vocab, cols]; padding_idx < 0: none; workspace: a byte
+    tensor of workspace_bytes()."""
     vocab, cols = dweight.shape
     return L.EmbeddingBackwardArgs(_ptr(dy), _ptr(tokens), _ptr(dweight), tokens.numel(), vocab, cols, _row_stride(dy, cols),
-                                   _row_stride(dweight, cols), padding_idx, scale, element_type(dy), element_type(dweight),
-                                   index_type(tokens), _ptr(workspace), 0 if workspace is None else workspace.numel())
+                                   _row_stride(dweight, cols), padding_idx, scale, _code(dy), _code(dweight), _code(tokens),
+                                   _ptr(workspace), 0 if workspace is None else workspace.numel())
 
 
 def workspace_bytes(kernel_name: str, args) -> int:

@@ -29,9 +29,11 @@ float16, and are launched alone:
 from __future__ import annotations
 
 import math
-from contextlib import nullcontext
 from dataclasses import dataclass
+from numbers import Integral
 from typing import Any, Optional, Sequence, Tuple
+
+import torch
 
 from . import launcher as H
 
@@ -148,13 +150,12 @@ def histc(x, bins: int = 100, min: float = 0.0, max: float = 0.0) -> Op:
 
 
 # ------------------------------------------------------------------ token-model operators
-_DTYPES = ("float32", "bfloat16", "float16")
+_DTYPES = frozenset((torch.float32, torch.bfloat16, torch.float16))
 
 
 def _check_typed(x, what: str, name: str):
-    import torch
-    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise TypeError(f"{what}: {name} must be a CUDA tensor of {', '.join(_DTYPES)}")
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _DTYPES:
+        raise TypeError(f"{what}: {name} must be a float32, bfloat16 or float16 CUDA tensor")
 
 
 def _check_same_device(what: str, x, *others):
@@ -163,19 +164,18 @@ def _check_same_device(what: str, x, *others):
             raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
 
 
-def _as_rows(x, rows: int, cols: int):
-    """x as [rows, cols] with dense rows: a view where its strides allow it, else a contiguous copy."""
+def _as_rows(x, cols: int):
+    """x itself if it is contiguous; else a [rows, cols] view with dense rows where its strides allow one, or a contiguous copy."""
     if x.is_contiguous():
-        return x.view(rows, cols)
+        return x
     try:
-        v = x.view(rows, cols)
+        v = x.view(-1, cols)
     except RuntimeError:
-        return x.contiguous().view(rows, cols)
-    return v if cols == 1 or v.stride(1) == 1 else v.contiguous()
+        return x.contiguous()
+    return v if cols == 1 or v.stride(1) == 1 else x.contiguous()
 
 
 def _workspace(kernel: str, args, device):
-    import torch
     need = H.workspace_bytes(kernel, args)
     if not need:
         return None
@@ -185,7 +185,6 @@ def _workspace(kernel: str, args, device):
 
 
 def _check_tokens(tokens, what: str):
-    import torch
     if not isinstance(tokens, torch.Tensor) or not tokens.is_cuda or tokens.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{what}: tokens must be an int32 or int64 CUDA tensor")
     return tokens.contiguous()
@@ -202,7 +201,6 @@ def embedding(tokens, weight, scale: float = 1.0) -> Op:
     """scale * weight[tokens]: tokens [...] int32 / int64, weight [V, D] -> [..., D] of weight's type.
 
     A token outside [0, V), such as the -1 behind the last token of a padded sequence, looks up a row of zeros."""
-    import torch
     _check_typed(weight, "embedding", "weight")
     tok = _check_tokens(tokens, "embedding")
     if weight.dim() != 2 or weight.numel() == 0:
@@ -210,10 +208,9 @@ def embedding(tokens, weight, scale: float = 1.0) -> Op:
     scale = _check_scale(scale, "embedding")
     _check_same_device("embedding", weight, tok)
     vocab, cols = weight.shape
-    w = _as_rows(weight, vocab, cols)
-    out = torch.empty((tok.numel(), cols), device=weight.device, dtype=weight.dtype)
-    return Op("embedding_forward", H.embedding_args(tok, w, out, scale), (out.view(tokens.shape + (cols,)),), (tok, w, out),
-              weight.device)
+    w = _as_rows(weight, cols)
+    out = torch.empty((*tokens.shape, cols), device=weight.device, dtype=weight.dtype)
+    return Op("embedding_forward", H.embedding_args(tok, w, out, scale), (out,), (tok, w, out), weight.device)
 
 
 def embedding_backward(dy, tokens, num_embeddings: int, scale: float = 1.0, padding_idx: Optional[int] = None,
@@ -222,7 +219,6 @@ def embedding_backward(dy, tokens, num_embeddings: int, scale: float = 1.0, padd
 
     Row v is scale times the sum of the dy rows whose token is v, summed in 32 bits in the order of the tokens; the row of
     `padding_idx` is zeros, and the dy rows of that token and of tokens outside [0, num_embeddings) are not read."""
-    import torch
     what = "embedding_backward"
     _check_typed(dy, what, "dy")
     tok = _check_tokens(tokens, what)
@@ -239,21 +235,25 @@ def embedding_backward(dy, tokens, num_embeddings: int, scale: float = 1.0, padd
         raise TypeError(f"{what}: the gradient is of dy's type or float32")
     _check_same_device(what, dy, tok)
     cols = dy.shape[-1]
-    g = _as_rows(dy, tok.numel(), cols)
+    g = _as_rows(dy, cols)
     out = torch.empty((vocab, cols), device=dy.device, dtype=dtype)
     args = H.embedding_backward_args(g, tok, out, scale, -1 if padding_idx is None else int(padding_idx))
     return Op("embedding_backward", args, (out,), (tok, g, out, _workspace("embedding_backward", args, dy.device)), dy.device)
 
 
 def _norm_shape(x, normalized_shape, what: str) -> Tuple[int, ...]:
-    shape = (int(normalized_shape),) if isinstance(normalized_shape, int) else tuple(int(n) for n in normalized_shape)
+    if isinstance(normalized_shape, int):
+        if x.dim() and x.shape[-1] == normalized_shape and normalized_shape > 0:
+            return (normalized_shape,)
+        shape = (normalized_shape,)
+    else:
+        shape = (int(normalized_shape),) if isinstance(normalized_shape, Integral) else tuple(int(n) for n in normalized_shape)
     if not shape or x.dim() < len(shape) or tuple(x.shape[-len(shape):]) != shape or math.prod(shape) == 0:
         raise ValueError(f"{what}: normalized_shape {shape} is not the (non-empty) end of the input's shape {tuple(x.shape)}")
     return shape
 
 
 def _norm_param(p, x, shape, what: str, name: str):
-    import torch
     if p is None:
         return None
     _check_typed(p, what, name)
@@ -268,7 +268,6 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps: float = 1e-5) -
     """torch.native_layer_norm: x [..., *normalized_shape] -> (y, mean, rstd), mean and rstd float32 [..., 1, ...].
 
     weight and bias are both of x's type or both float32; y is of x's type."""
-    import torch
     what = "layer_norm"
     _check_typed(x, what, "x")
     shape = _norm_shape(x, normalized_shape, what)
@@ -280,14 +279,13 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps: float = 1e-5) -
         raise ValueError(f"{what}: eps must be finite and not negative")
     _check_same_device(what, x, w, b)
     cols = math.prod(shape)
-    rows = x.numel() // cols
-    x2 = _as_rows(x, rows, cols)
-    y = torch.empty((rows, cols), device=x.device, dtype=x.dtype)
-    mean = torch.empty(rows, device=x.device, dtype=torch.float32)
-    rstd = torch.empty(rows, device=x.device, dtype=torch.float32)
-    stat = tuple(x.shape[:x.dim() - len(shape)]) + (1,) * len(shape)
-    return Op("layer_norm_forward", H.layer_norm_args(x2, y, w, b, mean, rstd, eps),
-              (y.view(x.shape), mean.view(stat), rstd.view(stat)), (x2, w, b, y, mean, rstd), x.device)
+    stat = (*x.shape[:x.dim() - len(shape)], *(1,) * len(shape))
+    x2 = _as_rows(x, cols)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    mean = torch.empty(stat, device=x.device, dtype=torch.float32)
+    rstd = torch.empty(stat, device=x.device, dtype=torch.float32)
+    return Op("layer_norm_forward", H.layer_norm_args(x2, y, w, b, mean, rstd, eps, cols), (y, mean, rstd),
+              (x2, w, b, y, mean, rstd), x.device)
 
 
 def layer_norm_backward(dy, x, normalized_shape, mean, rstd, weight=None,
@@ -296,7 +294,6 @@ def layer_norm_backward(dy, x, normalized_shape, mean, rstd, weight=None,
 
     `output_mask` says which of the three are wanted, the others come back as None (default: dx, and the parameters'
     gradients where there is a weight).  dweight and dbias are of weight's type (x's without one)."""
-    import torch
     what = "layer_norm_backward"
     _check_typed(x, what, "x")
     _check_typed(dy, what, "dy")
@@ -315,14 +312,13 @@ def layer_norm_backward(dy, x, normalized_shape, mean, rstd, weight=None,
     if len(mask) != 3 or not any(mask):
         raise ValueError(f"{what}: output_mask must be three flags, one of them set")
     _check_same_device(what, x, dy, mean, rstd, w)
-    dy2, x2, mean, rstd = _as_rows(dy, rows, cols), _as_rows(x, rows, cols), mean.contiguous(), rstd.contiguous()
+    dy2, x2, mean, rstd = _as_rows(dy, cols), _as_rows(x, cols), mean.contiguous(), rstd.contiguous()
     ptype = x.dtype if w is None else w.dtype
-    dx = torch.empty((rows, cols), device=x.device, dtype=x.dtype) if mask[0] else None
-    dw = torch.empty(cols, device=x.device, dtype=ptype) if mask[1] else None
-    db = torch.empty(cols, device=x.device, dtype=ptype) if mask[2] else None
-    args = H.layer_norm_backward_args(dy2, x2, mean, rstd, w, dx, dw, db)
-    return Op("layer_norm_backward", args,
-              (dx if dx is None else dx.view(x.shape), dw if dw is None else dw.view(shape), db if db is None else db.view(shape)),
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if mask[0] else None
+    dw = torch.empty(shape, device=x.device, dtype=ptype) if mask[1] else None
+    db = torch.empty(shape, device=x.device, dtype=ptype) if mask[2] else None
+    args = H.layer_norm_backward_args(dy2, x2, mean, rstd, w, dx, dw, db, cols=cols)
+    return Op("layer_norm_backward", args, (dx, dw, db),
               (dy2, x2, mean, rstd, w, dx, dw, db, _workspace("layer_norm_backward", args, x.device)), x.device)
 
 
@@ -404,16 +400,19 @@ def run(op: Op, stream=None):
 
 
 def _run_on_device(op: Op, stream):
-    import torch
     index = op.device.index
-    with nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index):
-        H.launch_native(op.kernel, op.args, stream=stream)
-        if stream is not None:
-            used = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream), device=op.device)
-            if used != torch.cuda.current_stream():
-                for t in op.keep:
-                    if t is not None:
-                        t.record_stream(used)
+    if stream is None and torch.cuda.current_device() == index:
+        H.launch_native(op.kernel, op.args, stream=torch._C._cuda_getCurrentRawStream(index))   # (current_stream() without its object)
+        return op.outputs
+    current = torch.cuda.current_stream(op.device)
+    used = current if stream is None else stream if isinstance(stream, torch.cuda.Stream) else \
+        torch.cuda.ExternalStream(int(stream), device=op.device)
+    with torch.cuda.device(op.device):
+        H.launch_native(op.kernel, op.args, stream=used)
+    if used != current:
+        for t in op.keep:
+            if t is not None:
+                t.record_stream(used)
     return op.outputs
 
 
