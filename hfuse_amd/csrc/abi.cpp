@@ -504,7 +504,7 @@ int prepare_blake2b(const hf_blake2b_args &a, bool sia, const SearchConstants &c
 
 // `consts`: the constants a search kernel is launched with; null = the process-wide set as it is now.
 // ------------------------------------------------ token-model operators
-constexpr int64_t kMaxCols = (int64_t)1 << 28;   // a row's bytes and lanes are counted in 32 bits
+constexpr int64_t kMaxCols = (int64_t)1 << 27;   // a row's bytes and the threads of a grid over it are counted in 32 bits
 bool element_type_ok(int t) { return t == HF_F32 || t == HF_BF16 || t == HF_F16; }
 size_t element_bytes(int t) { return t == HF_F32 ? 4 : 2; }
 bool aligned_to(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -538,7 +538,7 @@ int check_norm_sizes(const std::string &who, const A &a) {
   if (a.param_type != a.type && a.param_type != HF_F32)
     return fail(HF_EINVAL, who + "parameters must be of the rows' type or float32");
   if (a.rows < 0 || !extent_ok(a.cols)) return fail(HF_EINVAL, who + "negative row count or no columns");
-  if (a.rows >= kMaxExtent || a.cols >= kMaxCols) return fail(HF_EUNSUPPORTED, who + "2^31 rows or 2^28 columns are not built");
+  if (a.rows >= kMaxExtent || a.cols >= kMaxCols) return fail(HF_EUNSUPPORTED, who + "2^31 rows or 2^27 columns are not built");
   return HF_OK;
 }
 template <class A>
@@ -547,7 +547,7 @@ int check_embedding_sizes(const std::string &who, const A &a) {
   if (a.index_type != HF_I32 && a.index_type != HF_I64) return fail(HF_EINVAL, who + "unknown token type");
   if (a.ntokens < 0 || !extent_ok(a.vocab) || !extent_ok(a.cols))
     return fail(HF_EINVAL, who + "negative token count, no vocabulary or no columns");
-  if (a.ntokens >= kMaxExtent || a.cols >= kMaxCols) return fail(HF_EUNSUPPORTED, who + "2^31 tokens or 2^28 columns are not built");
+  if (a.ntokens >= kMaxExtent || a.cols >= kMaxCols) return fail(HF_EUNSUPPORTED, who + "2^31 tokens or 2^27 columns are not built");
   if (!std::isfinite(a.scale)) return fail(HF_EINVAL, who + "scale must be finite");
   return HF_OK;
 }

@@ -11,31 +11,32 @@ namespace {
 template <class T, class I, int VEC, int U>
 __global__ __launch_bounds__(256) void embedding_kernel(hf_embedding_args a, int lanes_log2, unsigned tiles) {
   const unsigned lanes = 1u << lanes_log2, lane = threadIdx.x & (lanes - 1);
-  const unsigned long long group = ((unsigned long long)blockIdx.x * 256u + threadIdx.x) >> lanes_log2;
-  const int64_t i = (int64_t)(group / tiles);
-  const int tile = (int)(group % tiles);
-  if (i >= a.ntokens) return;
-  const int64_t t = (int64_t) static_cast<const I *>(a.tokens)[i];
-  const bool used = t >= 0 && t < a.vocab;
-  const T *w = static_cast<const T *>(a.weight) + (used ? t : 0) * a.weight_stride;
-  T *out = static_cast<T *>(a.out) + i * a.out_stride;
   const int cols = (int)a.cols, slots = row_slots<VEC>(cols);
-  int col[U];
-  vec_t<T, VEC> v[U];
+  const unsigned long long groups = (unsigned long long)a.ntokens * tiles, step = ((unsigned long long)gridDim.x * 256u) >> lanes_log2;
+  for (unsigned long long group = ((unsigned long long)blockIdx.x * 256u + threadIdx.x) >> lanes_log2; group < groups; group += step) {
+    const int64_t i = (int64_t)(group / tiles);
+    const int first = (int)(group % tiles) * U * (int)lanes + (int)lane;
+    const int64_t t = (int64_t) static_cast<const I *>(a.tokens)[i];
+    const bool used = t >= 0 && t < a.vocab;
+    const T *w = static_cast<const T *>(a.weight) + (used ? t : 0) * a.weight_stride;
+    T *out = static_cast<T *>(a.out) + i * a.out_stride;
+    int col[U];
+    vec_t<T, VEC> v[U];
 #pragma unroll
-  for (int u = 0; u < U; u++) {
-    col[u] = slot_column<VEC>(min((tile * U + u) * (int)lanes + (int)lane, slots - 1), cols);   // (lanes behind the row repeat its last slot)
-    v[u] = used ? load_vec<T, VEC>(w + col[u]) : (vec_t<T, VEC>)(T)0.0f;
-  }
-#pragma unroll
-  for (int u = 0; u < U; u++) {
-    if (a.scale != 1.0f) {   // (1: the table's bits)
-      float f[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; e++) f[e] = elem<T, VEC>(v[u], e) * a.scale;
-      v[u] = round_vec<T, VEC>(f);
+    for (int u = 0; u < U; u++) {
+      col[u] = slot_column<VEC>(min(first + u * (int)lanes, slots - 1), cols);   // (lanes behind the row repeat its last slot)
+      v[u] = used ? load_vec<T, VEC>(w + col[u]) : (vec_t<T, VEC>)(T)0.0f;
     }
-    if ((tile * U + u) * (int)lanes + (int)lane < slots) store_vec_stream<T, VEC>(out + col[u], v[u]);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (a.scale != 1.0f) {   // (1: the table's bits)
+        float f[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) f[e] = elem<T, VEC>(v[u], e) * a.scale;
+        v[u] = round_vec<T, VEC>(f);
+      }
+      if (first + u * (int)lanes < slots) store_vec_stream<T, VEC>(out + col[u], v[u]);
+    }
   }
 }
 
@@ -522,7 +523,7 @@ TablePlan plan_table(const hf_embedding_backward_args &a, int cus) {
   const int64_t row_bytes = a.cols * (a.out_type == HF_F32 ? 4 : 2);
   p.zero_log2 = 0;   // lanes to a row of zeros: as many as it has 16-byte stores, a workgroup at most
   while (p.zero_log2 < 8 && ((int64_t)16 << p.zero_log2) < row_bytes) p.zero_log2++;
-  while (p.zero_log2 > 0 && (a.vocab << p.zero_log2) >= (int64_t)1 << 31) p.zero_log2--;
+  while (p.zero_log2 > 0 && (a.vocab << p.zero_log2) >= (int64_t)1 << 31) p.zero_log2--;   // lanes are numbered in 32 bits
   size_t at = 16;
   auto take = [&at](size_t bytes) {
     const size_t here = at;
@@ -562,6 +563,7 @@ hipError_t sort_tokens(const hf_embedding_backward_args &a, const TablePlan &p, 
   if (a.ntokens <= kSortStep) {
     const int64_t row_bytes = a.cols * (int64_t)all.element;
     int64_t rows = std::max<int64_t>(1, std::min<int64_t>(kFewRows, kFewBytes / row_bytes));
+    while (a.vocab / rows >= 1 << 23) rows *= 2;   // a grid has less than 2^32 threads (kFewRows rows: vocab < 2^31)
     const unsigned blocks = (unsigned)((a.vocab + rows - 1) / rows);
     hipLaunchKernelGGL((sort_few_kernel<I>), dim3(1 + blocks), dim3(kSortThreads), 0, s, a, sc, p.passes, p.digit_bits, (unsigned)rows, all);
     return hipGetLastError();
@@ -631,7 +633,7 @@ namespace {
 template <class T, class I, int VEC, int U>
 hipError_t look_up(const hf_embedding_args &a, int lanes_log2, hipStream_t s) {
   const int64_t slots = (a.cols + VEC - 1) / VEC, per_tile = (int64_t)U << lanes_log2, tiles = (slots + per_tile - 1) / per_tile;
-  const int64_t blocks = (((a.ntokens * tiles) << lanes_log2) + 255) / 256;
+  const int64_t blocks = std::min<int64_t>((((a.ntokens * tiles) << lanes_log2) + 255) / 256, 1 << 23);   // a grid has less than 2^32 threads
   hipLaunchKernelGGL((embedding_kernel<T, I, VEC, U>), dim3((unsigned)blocks), dim3(256), 0, s, a, lanes_log2, (unsigned)tiles);
   return hipGetLastError();
 }

@@ -392,7 +392,11 @@ def _ptr(t):
 
 def _row_stride(t, cols: int) -> int:
     """Elements between the rows of `cols` elements of a contiguous tensor, or of a [rows, cols] one with dense rows."""
-    return cols if t is None or t.is_contiguous() else t.stride(0)
+    if t is None or t.is_contiguous():
+        return cols
+    if t.dim() != 2 or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
+        raise ValueError("rows must be dense: a contiguous tensor, or [rows, cols] with adjacent columns")
+    return t.stride(0)
 
 
 def layer_norm_args(x, y, weight=None, bias=None, mean=None, rstd=None, eps: float = 1e-5, cols: int = 0) -> L.LayerNormArgs:

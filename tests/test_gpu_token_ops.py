@@ -413,6 +413,17 @@ def test_long_offsets(cuda):
     assert (dbias[::2] == 6).all() and (dbias[1::2] == 8).all() and not dx[:-2].any()
 
 
+def test_more_lanes_than_a_grid_has_threads(cuda):
+    """Rows of five elements take eight lanes each: 2^29 tokens and some are more than 2^32 lanes."""
+    n = (1 << 29) + 1000
+    tok = torch.zeros(n, device=cuda, dtype=torch.int32)
+    tok[-1], tok[-2], tok[1 << 29] = 2, -1, 1
+    w = torch.arange(15, device=cuda).view(3, 5).to(torch.bfloat16) + 1
+    (out,) = ops.run(ops.embedding(tok, w))
+    assert torch.equal(out[-1], w[2]) and not out[-2].any() and torch.equal(out[1 << 29], w[1]) and torch.equal(out[-3], w[0])
+    assert torch.equal(out[(1 << 29) - 1], w[0]) and torch.equal(out[5], w[0])
+
+
 def test_empty_batches(cuda):
     w = rand((9, 16), 31).to(cuda)
     none = torch.zeros((2, 0), dtype=torch.int64, device=cuda)

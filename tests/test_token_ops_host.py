@@ -46,7 +46,7 @@ def lookup_grad(**kw):
 
 BAD = [
     ("layer_norm_forward", norm, [dict(x=None), dict(y=None), dict(x=P + 2), dict(y=P + 1), dict(weight=P + 2), dict(mean=P + 1),
-                                  dict(rows=-1), dict(rows=1 << 31), dict(cols=0), dict(cols=1 << 31), dict(cols=1 << 28), dict(x_stride=-64),
+                                  dict(rows=-1), dict(rows=1 << 31), dict(cols=0), dict(cols=1 << 31), dict(cols=1 << 27), dict(x_stride=-64),
                                   dict(y_stride=63), dict(x_stride=1 << 62), dict(eps=-1.0), dict(eps=float("nan")),
                                   dict(eps=float("inf")), dict(type=3), dict(type=-1), dict(type=L.HF_F32, param_type=L.HF_F16),
                                   dict(type=L.HF_BF16, param_type=L.HF_F16)]),
@@ -57,7 +57,7 @@ BAD = [
                                    dict(weight_stride=-1), dict(ntokens=-1), dict(ntokens=1 << 31), dict(vocab=0), dict(cols=0),
                                    dict(scale=float("inf")), dict(scale=float("nan")), dict(type=4), dict(index_type=2)]),
     ("embedding_backward", lookup_grad, [dict(dy=None), dict(tokens=None), dict(dweight=None), dict(dweight_stride=63), dict(dy_stride=-2),
-                                         dict(padding_idx=10), dict(ntokens=-1), dict(vocab=-1), dict(vocab=1 << 31), dict(cols=0), dict(cols=1 << 28), dict(ntokens=1 << 31),
+                                         dict(padding_idx=10), dict(ntokens=-1), dict(vocab=-1), dict(vocab=1 << 31), dict(cols=0), dict(cols=1 << 27), dict(ntokens=1 << 31),
                                          dict(scale=float("nan")), dict(type=L.HF_F32, out_type=L.HF_F16),
                                          dict(type=L.HF_BF16, out_type=L.HF_F16), dict(index_type=-1), dict(tokens=P + 2)]),
 ]
@@ -118,3 +118,14 @@ def test_operators_refuse_cpu_tensors():
                  lambda: ops.embedding_backward(x, t, 10)):
         with pytest.raises(TypeError):
             make()
+
+
+def test_argument_builders_refuse_rows_that_are_not_dense():
+    y = torch.zeros(4, 6)
+    for x in (torch.zeros(6, 4).t(), torch.zeros(2, 4, 6).transpose(0, 1), torch.zeros(4, 12)[:, ::2]):
+        with pytest.raises(ValueError):
+            H.layer_norm_args(x, y)
+    a = H.layer_norm_args(torch.zeros(4, 9)[:, :6], y)
+    assert (a.rows, a.cols, a.x_stride, a.y_stride) == (4, 6, 9, 6)
+    a = H.layer_norm_args(torch.zeros(2, 3, 6), torch.zeros(2, 3, 6), cols=18)
+    assert (a.rows, a.cols, a.x_stride) == (2, 18, 18)
