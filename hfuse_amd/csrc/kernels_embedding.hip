@@ -140,6 +140,7 @@ __device__ __forceinline__ unsigned rank_equal(unsigned digit, bool used, int bi
 }
 
 // Inclusive sum over the threads of a workgroup in their order, and the sum of all; one barrier.
+template <int WAVES>
 __device__ __forceinline__ unsigned scan_block(unsigned v, unsigned *part, unsigned &all) {
   const unsigned lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -151,7 +152,7 @@ __device__ __forceinline__ unsigned scan_block(unsigned v, unsigned *part, unsig
   __syncthreads();
   all = 0;
 #pragma unroll
-  for (unsigned w = 0; w < kSortWaves; w++) {
+  for (unsigned w = 0; w < WAVES; w++) {
     if (w < wave) v += part[w];
     all += part[w];
   }
@@ -212,17 +213,27 @@ __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(hf_embedding
   constexpr int kOwn = kMaxBuckets / kSortThreads;   // buckets 2 tid and 2 tid + 1 are this thread's
   unsigned before[kOwn] = {0, 0}, total[kOwn] = {0, 0};
   if (tid * kOwn < buckets) {   // (one bit: two buckets)
-#pragma unroll 8
-    for (unsigned t = 0; t < sc.tiles; t++) {
-      const uint2 c = *reinterpret_cast<const uint2 *>(sc.counts + t * buckets + tid * kOwn);
-      before[0] += t < blockIdx.x ? c.x : 0;
-      before[1] += t < blockIdx.x ? c.y : 0;
-      total[0] += c.x;
-      total[1] += c.y;
+    constexpr unsigned kAhead = 8;   // counts on their way at once (the registers of 16 cost the rows of zeros a tenth of their rate)
+    for (unsigned t = 0; t < sc.tiles; t += kAhead) {
+      uint2 c[kAhead];
+#pragma unroll
+      for (unsigned i = 0; i < kAhead; i++)
+        c[i] = *reinterpret_cast<const uint2 *>(sc.counts + min(t + i, sc.tiles - 1) * buckets + tid * kOwn);
+#pragma unroll
+      for (unsigned i = 0; i < kAhead; i++) {
+        if (t + i < blockIdx.x) {
+          before[0] += c[i].x;
+          before[1] += c[i].y;
+        }
+        if (t + i < sc.tiles) {
+          total[0] += c[i].x;
+          total[1] += c[i].y;
+        }
+      }
     }
   }
   unsigned all;
-  const unsigned upto = scan_block(total[0] + total[1], scan, all);
+  const unsigned upto = scan_block<kSortWaves>(total[0] + total[1], scan, all);
   if (tid * kOwn < buckets) {
     base[tid * kOwn] = upto - total[0] - total[1] + before[0];
     base[tid * kOwn + 1] = upto - total[1] + before[1];
@@ -259,31 +270,32 @@ __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(hf_embedding
   }
 }
 
-// Few tokens (kSortStep at most), one launch: workgroup 0 sorts them in its LDS, digit by digit; the others have `rows` rows
-// of the table each, look through the tokens themselves and write the rows of zeros.
-constexpr unsigned kFewRows = 256;   // rows of a workgroup at most
-template <class I>
-__global__ __launch_bounds__(kSortThreads) void sort_few_kernel(hf_embedding_backward_args a, TableScratch sc, int passes, int bits, unsigned rows,
-                                                                ZeroRows z) {
-  __shared__ uint2 list[kSortStep];
-  __shared__ unsigned count[kSortWaves][kMaxBuckets], scan[kSortWaves];
+// Few tokens (64 WAVES KEYS at most), one launch: workgroup 0 sorts them in its LDS, digit by digit; the others have `rows`
+// rows of the table each, look through the tokens themselves and write the rows of zeros.
+template <class I, int WAVES, int KEYS>
+__global__ __launch_bounds__(64 * WAVES) void sort_few_kernel(hf_embedding_backward_args a, TableScratch sc, int passes, int bits, unsigned rows,
+                                                              ZeroRows z) {
+  constexpr unsigned kThreads = 64 * WAVES;
+  constexpr int kOwn = (kMaxBuckets + kThreads - 1) / kThreads;   // buckets of a thread
+  __shared__ uint2 list[kThreads * KEYS];
+  __shared__ unsigned count[WAVES][kMaxBuckets], scan[WAVES];
   const unsigned tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  uint2 entry[kSortKeys];
+  uint2 entry[KEYS];
 #pragma unroll
-  for (int u = 0; u < kSortKeys; u++) entry[u] = list_entry<I, true>(a, nullptr, (wave * kSortKeys + u) * 64u + lane, (unsigned)a.ntokens);
+  for (int u = 0; u < KEYS; u++) entry[u] = list_entry<I, true>(a, nullptr, (wave * KEYS + u) * 64u + lane, (unsigned)a.ntokens);
   if (blockIdx.x > 0) {
-    unsigned *present = count[0];
+    unsigned *present = count[0];   // a flag a row, kThreads of them at most
     const size_t first = (size_t)(blockIdx.x - 1) * rows;
     const unsigned mine = (unsigned)min((size_t)rows, (size_t)a.vocab - first);
-    if (tid < kFewRows) present[tid] = 0;
+    present[tid] = 0;
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kSortKeys; u++) {
+    for (int u = 0; u < KEYS; u++) {
       const size_t r = (size_t)entry[u].y - first;
       if (entry[u].y != ~0u && r < mine) present[r] = 1;
     }
     __syncthreads();
-    for (unsigned r = tid >> z.lanes_log2; r < mine; r += kSortThreads >> z.lanes_log2)
+    for (unsigned r = tid >> z.lanes_log2; r < mine; r += kThreads >> z.lanes_log2)
       if (!present[r]) zero_row(a, z, first + r, tid & ((1u << z.lanes_log2) - 1u));
     return;
   }
@@ -292,51 +304,57 @@ __global__ __launch_bounds__(kSortThreads) void sort_few_kernel(hf_embedding_bac
   for (int pass = 0; pass < passes; pass++) {
     const int shift = pass * bits;
     for (unsigned b = lane; b < buckets; b += 64) count[wave][b] = 0;   // a wave's counters are its own
-    unsigned rank[kSortKeys];
+    unsigned rank[KEYS];
 #pragma unroll
-    for (int u = 0; u < kSortKeys; u++)
+    for (int u = 0; u < KEYS; u++)
       rank[u] = rank_equal((entry[u].y >> shift) & (buckets - 1), entry[u].y != ~0u, bits, lane, count[wave]);
     __syncthreads();
-    constexpr int kOwn = kMaxBuckets / kSortThreads;
     unsigned total = 0;
-    if (tid * kOwn < buckets)
-      for (int o = 0; o < kOwn; o++)
-        for (int w = 0; w < kSortWaves; w++) total += count[w][tid * kOwn + o];
-    unsigned at = scan_block(total, scan, used) - total;
-    if (tid * kOwn < buckets)
-      for (int o = 0; o < kOwn; o++)
-        for (int w = 0; w < kSortWaves; w++) {
-          const unsigned c = count[w][tid * kOwn + o];
-          count[w][tid * kOwn + o] = at;
-          at += c;
-        }
+    for (unsigned b = tid * kOwn; b < min((tid + 1) * kOwn, buckets); b++)
+      for (int w = 0; w < WAVES; w++) total += count[w][b];
+    unsigned at = scan_block<WAVES>(total, scan, used) - total;
+    for (unsigned b = tid * kOwn; b < min((tid + 1) * kOwn, buckets); b++)
+      for (int w = 0; w < WAVES; w++) {
+        const unsigned c = count[w][b];
+        count[w][b] = at;
+        at += c;
+      }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kSortKeys; u++)
+    for (int u = 0; u < KEYS; u++)
       if (entry[u].y != ~0u) list[count[wave][(entry[u].y >> shift) & (buckets - 1)] + rank[u]] = entry[u];
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kSortKeys; u++) {
-      const unsigned i = (wave * kSortKeys + u) * 64u + lane;
+    for (int u = 0; u < KEYS; u++) {
+      const unsigned i = (wave * KEYS + u) * 64u + lane;
       entry[u] = i < used ? list[i] : make_uint2(0, ~0u);
     }
     __syncthreads();   // the list and the counters are written again
   }
 #pragma unroll
-  for (int u = 0; u < kSortKeys; u++)
-    if (entry[u].y != ~0u) sc.order[(wave * kSortKeys + u) * 64u + lane] = entry[u];
+  for (int u = 0; u < KEYS; u++)
+    if (entry[u].y != ~0u) sc.order[(wave * KEYS + u) * 64u + lane] = entry[u];
   if (tid == 0) {
     sc.state[0] = used;
     sc.state[1] = 0;
   }
 }
 
-// First entry of [lo, hi) whose token is larger than `id` (hi if there is none); the list is sorted.
+// First entry of [lo, hi) whose token is larger than `id` (hi if there is none); the list is sorted.  The ones up to `id`
+// are counted, 64 at a time by a whole wave and 8 by a thread: a chunk's worth takes one wait for memory or a few.
+template <bool WIDE>
 __device__ __forceinline__ unsigned first_above(const uint2 *order, unsigned lo, unsigned hi, unsigned id) {
   while (lo < hi) {
-    const unsigned mid = (lo + hi) / 2;
-    if (order[mid].y > id) hi = mid;
-    else lo = mid + 1;
+    unsigned n = 0;
+    if constexpr (WIDE) {
+      const unsigned at = lo + (threadIdx.x & 63u);
+      n = (unsigned)__builtin_popcountll(__ballot(at < hi && order[min(at, hi - 1)].y <= id));
+    } else {
+#pragma unroll
+      for (unsigned i = 0; i < 8; i++) n += lo + i < hi && order[min(lo + i, hi - 1)].y <= id;
+    }
+    lo += n;
+    if (n < (WIDE ? 64 : 8)) break;
   }
   return lo;
 }
@@ -362,8 +380,8 @@ __global__ __launch_bounds__(256) void sum_rows_kernel(hf_embedding_backward_arg
   const bool starts = !(cont0 && idl == id0);
   const bool shared0 = cont0 && ((crosses && idl == id0) || (k0 > sc.chunk && order[k0 - sc.chunk - 1].y == id0));
   const bool sharedl = starts && crosses && k1 + sc.chunk < used && order[k1 + sc.chunk].y == idl;
-  const unsigned begin = cont0 && !shared0 ? first_above(order, k0, k1, id0) : k0;   // the rest of that token is the other chunk's
-  const unsigned end = starts && crosses && !sharedl ? first_above(order, k1, min(k1 + sc.chunk, used), idl) : k1;
+  const unsigned begin = cont0 && !shared0 ? first_above<WIDE>(order, k0, k1, id0) : k0;   // the rest of that token is the other chunk's
+  const unsigned end = starts && crosses && !sharedl ? first_above<WIDE>(order, k1, min(k1 + sc.chunk, used), idl) : k1;
   if (tile == 0 && lane == 0) {
     if (sharedl) sc.shared[atomicAdd(&sc.state[1], 1u)] = c;   // in any order: each is joined by itself
     if (shared0 && !(crosses && idl == id0)) sc.last[id0] = c;
@@ -396,69 +414,54 @@ __global__ __launch_bounds__(256) void sum_rows_kernel(hf_embedding_backward_arg
 #pragma unroll
     for (int e = 0; e < VEC; e++) acc[e] += elem<T, VEC>(row, e);
   };
-  constexpr int U = 4;   // rows on their way at once (twice that in a whole wave)
-  if constexpr (WIDE) {
-    // 64 entries at a time in the wave's lanes: a row's address is one v_readlane away, and the tokens' last rows are the
-    // bits of one ballot.  The next U rows are on their way while U are added.
-    for (unsigned base = begin; base < end; base += 64) {
-      const int m = (int)min(64u, end - base);
-      const uint2 mine = order[min(base + (unsigned)lane, end - 1)];
-      const unsigned behind = order[min(base + (unsigned)lane + 1, end - 1)].y;
-      const unsigned long long lasts = __ballot(behind != mine.y || base + (unsigned)lane + 1 >= end);
-      auto fetch = [&](vec_t<T, VEC> (&row)[U], int at) {
+  // As many entries as the group has lanes at a time, one in each: a row's address is one v_readlane (a whole wave) or one
+  // shuffle away, and the tokens' last rows are the bits of one ballot.  The next U rows are on their way while U are added.
+  constexpr int U = 4;
+  const int group_base = WIDE ? 0 : (int)(threadIdx.x & 63u) & ~(lanes - 1);
+  for (unsigned base = begin; base < end; base += (unsigned)lanes) {
+    const int m = (int)min((unsigned)lanes, end - base);
+    const uint2 mine = order[min(base + (unsigned)lane, end - 1)];
+    const unsigned behind = order[min(base + (unsigned)lane + 1, end - 1)].y;
+    const unsigned long long lasts = __ballot(behind != mine.y || base + (unsigned)lane + 1 >= end) >> group_base;
+    auto of_lane = [&](unsigned v, int i) {
+      return WIDE ? (unsigned)__builtin_amdgcn_readlane((int)v, i) : (unsigned)__shfl((int)v, group_base + i);
+    };
+    auto fetch = [&](vec_t<T, VEC> (&row)[U], int at) {
 #pragma unroll
-        for (int u = 0; u < U; u++)
-          row[u] = load_vec_stream<T, VEC>(dy + (size_t)(unsigned)__builtin_amdgcn_readlane((int)mine.x, min(at + u, m - 1)) * (size_t)a.dy_stride);
-      };
-      auto take = [&](const vec_t<T, VEC> (&row)[U], int at) {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-          if (at + u < m) {
-            add(row[u]);
-            if ((lasts >> (at + u)) & 1ull) put((unsigned)__builtin_amdgcn_readlane((int)mine.y, at + u));
-          }
-        }
-      };
-      vec_t<T, VEC> one[U], two[U];
-      fetch(one, 0);
-      for (int at = 0; at < m; at += 2 * U) {
-        fetch(two, at + U);
-        take(one, at);
-        if (at + 2 * U < m) fetch(one, at + 2 * U);
-        take(two, at + U);
-      }
-    }
-  } else {
-    for (unsigned k = begin; k < end; k += U) {
-      uint2 entry[U + 1];
-#pragma unroll
-      for (int u = 0; u <= U; u++) entry[u] = order[min(k + u, end - 1)];
-      vec_t<T, VEC> row[U];
-#pragma unroll
-      for (int u = 0; u < U; u++) row[u] = load_vec_stream<T, VEC>(dy + (size_t)entry[u].x * (size_t)a.dy_stride);
+      for (int u = 0; u < U; u++) row[u] = load_vec_stream<T, VEC>(dy + (size_t)of_lane(mine.x, min(at + u, m - 1)) * (size_t)a.dy_stride);
+    };
+    auto take = [&](const vec_t<T, VEC> (&row)[U], int at) {
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        if (k + u < end) {
+        if (at + u < m) {
           add(row[u]);
-          if (k + u + 1 == end || entry[u].y != entry[u + 1].y) put(entry[u].y);
+          if ((lasts >> (at + u)) & 1ull) put(of_lane(mine.y, at + u));
         }
       }
+    };
+    vec_t<T, VEC> one[U], two[U];
+    fetch(one, 0);
+    for (int at = 0; at < m; at += 2 * U) {
+      fetch(two, at + U);
+      take(one, at);
+      if (at + 2 * U < m) fetch(one, at + 2 * U);
+      take(two, at + U);
     }
   }
 }
 
-// The shared tokens: a workgroup adds up the parts of one token over 64 slots; its sixteen waves take the parts in turn
-// and their sums are added in the order of the waves.
-constexpr int kJoinWaves = 16;
-template <class O, int VEC>
-__global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(hf_embedding_backward_args a, TableScratch sc, unsigned tiles) {
-  __shared__ float sums[kJoinWaves][64 * VEC];
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+// The shared tokens: a workgroup adds up the parts of one token over one tile of slots.  Its groups of lanes (one a wave
+// where rows are wide) take the parts in turn and their sums are added in the order of the groups.
+template <class O, int VEC, int WAVES, bool WIDE>
+__global__ __launch_bounds__(64 * WAVES) void join_rows_kernel(hf_embedding_backward_args a, TableScratch sc, int lanes_log2, unsigned tiles) {
+  __shared__ float sums[WAVES][64 * VEC];
+  const int lanes = WIDE ? 64 : 1 << lanes_log2, lane = (int)threadIdx.x & (lanes - 1);
+  const unsigned group = WIDE ? threadIdx.x >> 6 : threadIdx.x >> lanes_log2, groups = WIDE ? WAVES : (64u * WAVES) >> lanes_log2;
   const int cols = (int)a.cols, slots = row_slots<VEC>(cols);
   const unsigned long long items = (unsigned long long)sc.state[1] * tiles;
   for (unsigned long long item = blockIdx.x; item < items; item += gridDim.x) {
     const unsigned c = sc.shared[item / tiles];
-    const int slot = (int)(item % tiles) * 64 + lane;
+    const int slot = (int)(item % tiles) * lanes + lane;
     const unsigned id = sc.order[(c + 1) * sc.chunk - 1].y;   // (a shared token fills the chunk behind: this one is full)
     const unsigned last = sc.last[id];
     const size_t width = (size_t)slots * VEC;
@@ -466,21 +469,25 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(hf_embedding
     float acc[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; e++) acc[e] = 0.0f;
-#pragma unroll 4
-    for (unsigned q = c + (unsigned)wave; q <= last; q += kJoinWaves) {
+#pragma unroll 8
+    for (unsigned q = c + group; q <= last; q += groups) {
       const vec_t<float, VEC> v = load_vec<float, VEC>(p + ((size_t)q * 2 + (q == c ? 1 : 0)) * width);
 #pragma unroll
       for (int e = 0; e < VEC; e++) acc[e] += elem<float, VEC>(v, e);
     }
+    if constexpr (!WIDE)   // the groups of a wave
+      for (int m = lanes; m < 64; m <<= 1)
 #pragma unroll
-    for (int e = 0; e < VEC; e++) sums[wave][e * 64 + lane] = acc[e];
+        for (int e = 0; e < VEC; e++) acc[e] += __shfl_xor(acc[e], m);
+#pragma unroll
+    for (int e = 0; e < VEC; e++) sums[threadIdx.x >> 6][e * 64 + ((int)threadIdx.x & 63)] = acc[e];
     __syncthreads();
-    if (wave == 0 && slot < slots) {
+    if (group == 0 && slot < slots) {
       float s[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; e++) {
         s[e] = 0.0f;
-        for (int w = 0; w < kJoinWaves; w++) s[e] += sums[w][e * 64 + lane];
+        for (int w = 0; w < WAVES; w++) s[e] += sums[w][e * 64 + lane];
         s[e] *= a.scale;
       }
       store_vec<O, VEC>(static_cast<O *>(a.dweight) + (size_t)id * (size_t)a.dweight_stride + slot_column<VEC>(slot, cols), round_vec<O, VEC>(s));
@@ -489,9 +496,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(hf_embedding
   }
 }
 
-constexpr int kMaxChunk = 64, kSumWaves = 16;   // entries of a chunk at most; waves a CU should have at least
-
-constexpr int64_t kFewBytes = 8192;   // bytes of the table to a workgroup of sort_few_kernel
+// Entries of a chunk at most, and the waves a CU should have at least before chunks are made smaller for more of them: a
+// small chunk shares more tokens out, which costs narrow rows more than the waves bring.
+constexpr int kMaxChunk = 64, kWideWaves = 16, kNarrowWaves = 4;
 
 // How the launches are cut: columns into slots and tiles, sorted entries into chunks, the token's bits into digits.
 struct TablePlan {
@@ -506,11 +513,11 @@ TablePlan plan_table(const hf_embedding_backward_args &a, int cus) {
   p.vec = a.cols >= vec ? vec : 1;
   p.slots = (int)((a.cols + p.vec - 1) / p.vec);
   p.lanes_log2 = 6;
-  while (p.lanes_log2 > 0 && (1 << (p.lanes_log2 - 1)) >= p.slots) p.lanes_log2--;
+  while (p.lanes_log2 > 3 && (1 << (p.lanes_log2 - 1)) >= p.slots) p.lanes_log2--;   // (eight lanes at least: they hold the entries)
   const int lanes = 1 << p.lanes_log2;
   p.col_tiles = (unsigned)((p.slots + lanes - 1) / lanes);
   p.chunk = kMaxChunk;
-  while (p.chunk > 8 && a.ntokens / p.chunk * p.col_tiles * lanes < (int64_t)cus * kSumWaves * 64) p.chunk /= 2;
+  while (p.chunk > 8 && a.ntokens / p.chunk * p.col_tiles * lanes < (int64_t)cus * (lanes == 64 ? kWideWaves : kNarrowWaves) * 64) p.chunk /= 2;
   while (a.ntokens / p.chunk * p.col_tiles * lanes >= (int64_t)1 << 31) p.chunk *= 2;   // lanes are numbered in 32 bits
   p.nchunks = (unsigned)((a.ntokens + p.chunk - 1) / p.chunk);
   int bits = 1;
@@ -521,8 +528,8 @@ TablePlan plan_table(const hf_embedding_backward_args &a, int cus) {
   p.tile = (unsigned)((steps + kSortTiles - 1) / kSortTiles * kSortStep);
   p.tiles = p.tile ? (unsigned)((a.ntokens + p.tile - 1) / p.tile) : 0;
   const int64_t row_bytes = a.cols * (a.out_type == HF_F32 ? 4 : 2);
-  p.zero_log2 = 0;   // lanes to a row of zeros: as many as it has 16-byte stores, a workgroup at most
-  while (p.zero_log2 < 8 && ((int64_t)16 << p.zero_log2) < row_bytes) p.zero_log2++;
+  p.zero_log2 = 0;   // lanes to a row of zeros: as many as it has 16-byte stores
+  while (((int64_t)16 << p.zero_log2) < row_bytes) p.zero_log2++;
   while (p.zero_log2 > 0 && (a.vocab << p.zero_log2) >= (int64_t)1 << 31) p.zero_log2--;   // lanes are numbered in 32 bits
   size_t at = 16;
   auto take = [&at](size_t bytes) {
@@ -552,22 +559,36 @@ hipError_t sum_tokens(const hf_embedding_backward_args &a, const TablePlan &p, c
     hipLaunchKernelGGL((sum_rows_kernel<T, O, VEC, false>), grid, dim3(256), 0, s, a, sc, p.lanes_log2, p.col_tiles);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.nchunks < 3) return e;   // a shared token crosses two chunk boundaries
-  const unsigned join_tiles = (unsigned)(p.slots + 63) / 64;
-  const unsigned joins = (unsigned)std::min<unsigned long long>((unsigned long long)p.nchunks * join_tiles, (unsigned long long)cus * 4);
-  hipLaunchKernelGGL((join_rows_kernel<O, VEC>), dim3(joins), dim3(64 * kJoinWaves), 0, s, a, sc, join_tiles);
+  const unsigned long long items = (unsigned long long)p.nchunks * p.col_tiles;
+  if (p.lanes_log2 == 6)
+    hipLaunchKernelGGL((join_rows_kernel<O, VEC, 16, true>), dim3((unsigned)std::min<unsigned long long>(items, (unsigned long long)cus * 4)), dim3(1024),
+                       0, s, a, sc, 6, p.col_tiles);
+  else
+    hipLaunchKernelGGL((join_rows_kernel<O, VEC, 4, false>), dim3((unsigned)std::min<unsigned long long>(items, (unsigned long long)cus * 16)), dim3(256),
+                       0, s, a, sc, p.lanes_log2, p.col_tiles);
+  return hipGetLastError();
+}
+
+// `bytes`: of the table to a workgroup, all of which look through the tokens.
+template <class I, int WAVES, int KEYS>
+hipError_t sort_few(const hf_embedding_backward_args &a, const TablePlan &p, const TableScratch &sc, const ZeroRows &all, int64_t bytes,
+                    hipStream_t s) {
+  constexpr int64_t kThreads = 64 * WAVES;
+  int64_t rows = std::max<int64_t>(1, std::min<int64_t>(kThreads, bytes / (a.cols * (int64_t)all.element)));
+  while (rows < kThreads && a.vocab / rows * kThreads >= (int64_t)1 << 31) rows = std::min(rows * 2, kThreads);   // a grid has less than 2^32 threads
+  ZeroRows z = all;
+  while (((int64_t)1 << z.lanes_log2) > kThreads) z.lanes_log2--;   // a workgroup's rows are its own
+  const unsigned blocks = (unsigned)((a.vocab + rows - 1) / rows);
+  hipLaunchKernelGGL((sort_few_kernel<I, WAVES, KEYS>), dim3(1 + blocks), dim3(kThreads), 0, s, a, sc, p.passes, p.digit_bits, (unsigned)rows, z);
   return hipGetLastError();
 }
 
 template <class I>
 hipError_t sort_tokens(const hf_embedding_backward_args &a, const TablePlan &p, const TableScratch &sc, const ZeroRows &all, hipStream_t s) {
-  if (a.ntokens <= kSortStep) {
-    const int64_t row_bytes = a.cols * (int64_t)all.element;
-    int64_t rows = std::max<int64_t>(1, std::min<int64_t>(kFewRows, kFewBytes / row_bytes));
-    while (a.vocab / rows >= 1 << 23) rows *= 2;   // a grid has less than 2^32 threads (kFewRows rows: vocab < 2^31)
-    const unsigned blocks = (unsigned)((a.vocab + rows - 1) / rows);
-    hipLaunchKernelGGL((sort_few_kernel<I>), dim3(1 + blocks), dim3(kSortThreads), 0, s, a, sc, p.passes, p.digit_bits, (unsigned)rows, all);
-    return hipGetLastError();
-  }
+  // One launch instead of two a digit: 24 against 30 us for 4096 tokens of a 2000 x 768 float32 table.  One workgroup's sort
+  // of more than 1024 tokens (11 us) is only worth it next to a small table (50000 x 2048 bf16: 54 against 52 us).
+  if (a.ntokens <= 1024) return sort_few<I, 4, 4>(a, p, sc, all, 8192, s);
+  if (a.ntokens <= 4096 && a.vocab * a.cols * (int64_t)all.element <= (int64_t)64 << 20) return sort_few<I, 8, 8>(a, p, sc, all, 65536, s);
   // the rows of zeros are shared evenly among the launches behind the first, which finds out what they are
   const unsigned parts = 2u * (unsigned)p.passes - 1u;
   ZeroRows z = {0, 0, all.lanes_log2, all.element};

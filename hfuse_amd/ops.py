@@ -175,11 +175,11 @@ def _as_rows(x, cols: int):
     return v if cols == 1 or v.stride(1) == 1 else x.contiguous()
 
 
-def _workspace(kernel: str, args, device):
+def _workspace(kernel: str, args, x):
     need = H.workspace_bytes(kernel, args)
     if not need:
         return None
-    ws = torch.empty(need, device=device, dtype=torch.uint8)
+    ws = x.new_empty(need, dtype=torch.uint8)
     args.workspace, args.workspace_bytes = ws.data_ptr(), need
     return ws
 
@@ -209,7 +209,7 @@ def embedding(tokens, weight, scale: float = 1.0) -> Op:
     _check_same_device("embedding", weight, tok)
     vocab, cols = weight.shape
     w = _as_rows(weight, cols)
-    out = torch.empty((*tokens.shape, cols), device=weight.device, dtype=weight.dtype)
+    out = weight.new_empty((*tokens.shape, cols))
     return Op("embedding_forward", H.embedding_args(tok, w, out, scale), (out,), (tok, w, out), weight.device)
 
 
@@ -236,9 +236,9 @@ def embedding_backward(dy, tokens, num_embeddings: int, scale: float = 1.0, padd
     _check_same_device(what, dy, tok)
     cols = dy.shape[-1]
     g = _as_rows(dy, cols)
-    out = torch.empty((vocab, cols), device=dy.device, dtype=dtype)
+    out = dy.new_empty((vocab, cols), dtype=dtype)
     args = H.embedding_backward_args(g, tok, out, scale, -1 if padding_idx is None else int(padding_idx))
-    return Op("embedding_backward", args, (out,), (tok, g, out, _workspace("embedding_backward", args, dy.device)), dy.device)
+    return Op("embedding_backward", args, (out,), (tok, g, out, _workspace("embedding_backward", args, dy)), dy.device)
 
 
 def _norm_shape(x, normalized_shape, what: str) -> Tuple[int, ...]:
@@ -282,8 +282,8 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps: float = 1e-5) -
     stat = (*x.shape[:x.dim() - len(shape)], *(1,) * len(shape))
     x2 = _as_rows(x, cols)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    mean = torch.empty(stat, device=x.device, dtype=torch.float32)
-    rstd = torch.empty(stat, device=x.device, dtype=torch.float32)
+    mean = x.new_empty(stat, dtype=torch.float32)
+    rstd = torch.empty_like(mean)
     return Op("layer_norm_forward", H.layer_norm_args(x2, y, w, b, mean, rstd, eps, cols), (y, mean, rstd),
               (x2, w, b, y, mean, rstd), x.device)
 
@@ -313,13 +313,11 @@ def layer_norm_backward(dy, x, normalized_shape, mean, rstd, weight=None,
         raise ValueError(f"{what}: output_mask must be three flags, one of them set")
     _check_same_device(what, x, dy, mean, rstd, w)
     dy2, x2, mean, rstd = _as_rows(dy, cols), _as_rows(x, cols), mean.contiguous(), rstd.contiguous()
-    ptype = x.dtype if w is None else w.dtype
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if mask[0] else None
-    dw = torch.empty(shape, device=x.device, dtype=ptype) if mask[1] else None
-    db = torch.empty(shape, device=x.device, dtype=ptype) if mask[2] else None
+    dw, db = ((x.new_empty(shape) if w is None else torch.empty_like(w)) if m else None for m in mask[1:])
     args = H.layer_norm_backward_args(dy2, x2, mean, rstd, w, dx, dw, db, cols=cols)
     return Op("layer_norm_backward", args, (dx, dw, db),
-              (dy2, x2, mean, rstd, w, dx, dw, db, _workspace("layer_norm_backward", args, x.device)), x.device)
+              (dy2, x2, mean, rstd, w, dx, dw, db, _workspace("layer_norm_backward", args, x)), x.device)
 
 
 # ------------------------------------------------------------------ nonce searches

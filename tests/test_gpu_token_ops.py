@@ -341,6 +341,24 @@ def test_embedding_backward_over_sizes(cuda, n, vocab):
     check_table_grad(dy, skewed, vocab, cuda, 0.5, 0, None, (n, vocab, "skewed"))
 
 
+@pytest.mark.parametrize("n", [900, 1030, 131073, 300007])
+@pytest.mark.parametrize("vocab", [512, 513, 400000, (1 << 27) + 5])
+def test_embedding_backward_long_lists_and_large_vocabularies(cuda, n, vocab):
+    """Sorts of one to four digits, of one workgroup's tokens to several steps a workgroup; compared on the rows named and
+    by the sum of all others."""
+    cols = 5 if vocab < 1 << 20 else 1
+    tok = (torch.rand((n,), generator=gen(n), dtype=torch.float64) ** 3 * vocab).long()
+    tok[::11], tok[n // 2:n // 2 + 200], tok[-1] = -1, 7, vocab - 1
+    dy = rand((n, cols), vocab % 1000)
+    (got,) = ops.run(ops.embedding_backward(dy.to(cuda), tok.to(cuda), vocab, 0.5))
+    got = got.cpu()
+    named, at = torch.unique(tok[tok >= 0], return_inverse=True)
+    want, tol = table_grad64(dy[tok >= 0], at, len(named), 0.5, None)
+    check(got[named], want, tol + half(torch.float32) * (want.abs() + tol) + floor(torch.float32), (n, vocab))
+    got[named] = 0
+    assert not got.any()
+
+
 @pytest.mark.parametrize("shape", ["one", "two ends", "last", "runs", "sorted", "reversed", "none"])
 def test_embedding_backward_token_patterns(cuda, shape):
     """All rows on one id, on the table's first and last, in runs longer and shorter than any tile, and no usable id at all."""
