@@ -7,7 +7,6 @@
 namespace hfuse {
 namespace {
 
-
 // LANES threads hold a row in registers, VPT slots of 16 bytes each: the row is read once, the mean and then the mean
 // square of the differences come from the registers, and the next row is on its way meanwhile.  A workgroup keeps its
 // weights in registers for all its rows.
@@ -182,6 +181,14 @@ hipError_t norm_forward(const hf_layer_norm_args &a, int cus, hipStream_t s) {
   if (slots <= 16) return norm_rows<T, P, VEC, 1, 16>(a, cus, s);
   if (slots <= 32) return norm_rows<T, P, VEC, 1, 32>(a, cus, s);
   if (slots <= 64) return norm_rows<T, P, VEC, 1, 64>(a, cus, s);
+  // Fewer rows than CUs: a row's latency is all there is, and one slot a thread is the shortest (us at 1 and 256 rows of
+  // bf16 against the forms below: 4096 columns 2.5 / 3.5 and 3.9 / 4.8, 1024 columns 2.4 / 2.6 and 3.3 / 3.5; from about
+  // 1000 rows on the others win: 4096 rows of 1024 columns 7.9 / 5.3).
+  if (a.rows <= cus) {
+    if (slots <= 256) return norm_rows<T, P, VEC, 1, 256>(a, cus, s);
+    if (slots <= 512) return norm_rows<T, P, VEC, 1, 512>(a, cus, s);
+    if (slots <= 1024) return norm_rows<T, P, VEC, 1, 1024>(a, cus, s);
+  }
   if (slots <= 128) return norm_rows<T, P, VEC, 2, 64>(a, cus, s);
   if (slots <= 256) return norm_rows<T, P, VEC, 4, 64>(a, cus, s);
   if (slots <= 512) return norm_rows<T, P, VEC, 4, 128>(a, cus, s);

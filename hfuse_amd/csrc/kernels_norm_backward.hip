@@ -7,7 +7,6 @@
 namespace hfuse {
 namespace {
 
-
 // One pass over the rows: LANES threads hold a row of x and of dy in registers, VPT slots of 16 bytes each, form the two
 // sums over the row that dx needs, write dx, and add dy * h and dy to the 32-bit sums of their columns, which stay in
 // registers for all rows of the workgroup.  The next row is on its way meanwhile.  A workgroup leaves one row of sums for

@@ -86,7 +86,7 @@ COLS = [1, 2, 7, 8, 63, 64, 65, 100, 257, 512, 1000, 1024, 1155, 2048, 2056, 409
 @pytest.mark.parametrize("cols", COLS)
 def test_layer_norm_over_row_lengths(cuda, type, cols):
     t = TYPES[type]
-    for rows, params in ((1, t), (5, torch.float32), (67, t)):
+    for rows, params in ((1, t), (5, torch.float32), (67, t), (300, torch.float32), (301, t)):
         x = rand((rows, cols), cols + rows, t, 2.0, 0.5)
         w, b = rand((cols,), 1, params, 0.2, 1.0), rand((cols,), 2, params)
         check_norm(x, w, b, 1e-5, run_norm(x, w, b, 1e-5, cuda), (type, cols, rows))
@@ -142,6 +142,8 @@ def test_layer_norm_hard_rows(cuda):
     w, b = rand((cols,), 12), rand((cols,), 13)
     got = run_norm(x, w, b, 1e-5, cuda)
     check_norm(x, w, b, 1e-5, got, "hard")
+    many = run_norm(x.repeat(40, 1), w, b, 1e-5, cuda)                                # the same rows among more of them
+    check_norm(x, w, b, 1e-5, [v[160:168] for v in many], "hard, many")
     assert torch.equal(got[0][2].cpu(), b)                                            # 0 * w + b
     bad = x.clone()
     bad[6, 17], bad[7, 999] = float("nan"), float("inf")
@@ -188,7 +190,7 @@ def run_grad(dy, x, mean, rstd, w, cuda, mask=None, put=lambda t: t):
 @pytest.mark.parametrize("cols", COLS)
 def test_layer_norm_backward_over_row_lengths(cuda, type, cols):
     t = TYPES[type]
-    for rows, params in ((1, t), (5, torch.float32), (67, t)):
+    for rows, params in ((1, t), (5, torch.float32), (67, t), (300, torch.float32), (301, t)):
         x, dy = rand((rows, cols), cols + rows, t, 2.0, 0.5), rand((rows, cols), cols, t, 0.1)
         w, (mean, rstd) = rand((cols,), 1, params, 0.2, 1.0), stats(x)
         got = run_grad(dy, x, mean, rstd, w, cuda)

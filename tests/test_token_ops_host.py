@@ -129,3 +129,53 @@ def test_argument_builders_refuse_rows_that_are_not_dense():
     assert (a.rows, a.cols, a.x_stride, a.y_stride) == (4, 6, 9, 6)
     a = H.layer_norm_args(torch.zeros(2, 3, 6), torch.zeros(2, 3, 6), cols=18)
     assert (a.rows, a.cols, a.x_stride) == (2, 18, 18)
+
+
+FUZZ = """
+import ctypes as C, random, sys
+ROOT = sys.argv[1]
+sys.path.insert(0, ROOT)
+import torch
+assert not torch.cuda.is_available()
+from hfuse_amd import _lib as L
+lib = L.lib()
+rng = random.Random(4711)
+VALS = [0, 1, 2, 3, 4, 7, 8, 64, 255, 256, 1024, 4096, 65536, -1, -2, 2**27 - 1, 2**27, 2**31 - 1, 2**31, 2**32, 2**40, 2**63 - 1, -2**63]
+P = 1 << 20
+LISTS = [(b"layer_norm_forward", lambda: L.LayerNormArgs(P, P, P, 2 * P, 3 * P, 3 * P, 4, 64, 64, 64, 1e-5, 1, 1)),
+         (b"layer_norm_backward", lambda: L.LayerNormBackwardArgs(P, P, P, P, P, 2 * P, 3 * P, 4 * P, 4, 64, 64, 64, 64, 1, 0, 8 * P, 1 << 62)),
+         (b"embedding_forward", lambda: L.EmbeddingArgs(P, P, 2 * P, 4, 10, 64, 64, 64, 1.0, 2, 1)),
+         (b"embedding_backward", lambda: L.EmbeddingBackwardArgs(P, P, 2 * P, 4, 10, 64, 64, 64, -1, 1.0, 1, 0, 1, 8 * P, 1 << 62))]
+seen = {}
+for i in range(20000):
+    name, make = rng.choice(LISTS)
+    a = make()
+    for field, kind in rng.sample(a._fields_, rng.randint(1, 4)):
+        if kind is C.c_float:
+            setattr(a, field, rng.choice((0.0, 1.0, -1.0, float("nan"), float("inf"))))
+        elif kind is C.c_int:
+            setattr(a, field, rng.randint(-1, 4))
+        else:
+            v = rng.choice(VALS)
+            setattr(a, field, v % 2**64 if kind in (C.c_void_p, C.c_size_t) else v)
+    n = C.c_size_t()
+    rc = lib.hf_workspace_bytes(name, C.byref(a), C.byref(n))
+    assert rc in (0, L.HF_EINVAL, L.HF_EUNSUPPORTED) and (rc == 0 or n.value == 0) and n.value < 1 << 50, (rc, n.value)
+    rc2 = lib.hf_launch_native(name, C.byref(a), 0, 0, None)
+    assert rc2 in (0, L.HF_EINVAL, L.HF_EUNSUPPORTED, L.HF_EHIP), rc2      # HF_EHIP: accepted, and no device to run on
+    assert rc == 0 or rc2 != 0
+    seen[rc2] = seen.get(rc2, 0) + 1
+assert seen[L.HF_EINVAL] > 2000 and seen[L.HF_EHIP] > 500, seen
+"""
+
+
+def test_mutated_argument_lists_never_crash():
+    """Accepted lists reach a launch that fails for want of a device: only where no GPU is visible."""
+    if torch.cuda.is_available():
+        pytest.skip("made-up pointers must not reach a GPU")
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FUZZ, root], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
