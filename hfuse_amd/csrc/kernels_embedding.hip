@@ -1,4 +1,9 @@
-// Token embedding: rows of a table by token id, scaled, and the gradient of the table.
+// Token embedding, out[i] = scale W[t_i], and the gradient of the table, dW[v] = scale sum of dy[i] over i with t_i = v.
+//
+// Both are bound by HBM.  Measured on an MI355X with 131072 tokens and a table of 128000 x 4096 bf16, ids of a learnt
+// vocabulary (the k-th with a probability of about 1 / k): lookup 263 us (1.07 GB written, 0.67 GB fetched for 0.27 GB of
+// distinct rows: 6.3 TB/s); gradient 370-405 us for 2.1 GB = 5.2-5.7 TB/s, of which the sort and the rows of zeros beside
+// it take 135, the sums 225, the shared tokens 11.
 #include <algorithm>
 
 #include "device/rows.h"
@@ -8,6 +13,8 @@ namespace hfuse {
 namespace {
 
 // A group of `lanes` lanes copies U of its slots of a row at once: all its reads are on their way before the first store.
+// (U 1 / 2 / 4 / 8: 337 / 276 / 270 / 301 us for the batch above, 4.6 / 4.8 / 5.4 / 7.4 us for 4999 rows of 1001 f16.)
+// Stores go past the caches, which keep the table's frequent rows (rows of 128 bf16: 87 -> 51 us for a million tokens).
 template <class T, class I, int VEC, int U>
 __global__ __launch_bounds__(256) void embedding_kernel(hf_embedding_args a, int lanes_log2, unsigned tiles) {
   const unsigned lanes = 1u << lanes_log2, lane = threadIdx.x & (lanes - 1);
@@ -45,7 +52,8 @@ __global__ __launch_bounds__(256) void embedding_kernel(hf_embedding_args a, int
 // for each digit), the dy rows of each token are summed from the sorted list (sum_rows_kernel), and tokens whose rows were
 // shared out are joined (join_rows_kernel).  The rows of zeros -- most of the table in a small batch -- are written by
 // further workgroups of the sort's launches: a sort of some thousand tokens waits for memory most of the time on a few
-// CUs and leaves the rest of the part and its write bandwidth to them.
+// CUs and leaves the rest of the part and its write bandwidth to them.  dy is read and the zeros are written past the
+// caches: otherwise the reads push the dirty zeros out of the memory-side cache and wait for them (sums 301 -> 224 us).
 // No floating-point atomics: every sum has one order, whatever the order in which workgroups run.
 
 constexpr int kSortWaves = 4;

@@ -1,4 +1,10 @@
-// Layer norm over the last dimension.
+// Layer norm over the last dimension: mean = sum(x) / n, var = sum((x - mean)^2) / n, y = (x - mean) / sqrt(var + eps) w + b.
+//
+// Bound by HBM: a row is read once and written once, about 8 operations an element (2 a byte in 16 bits).  Measured on an
+// MI355X: 32768 x 8192 bf16 with float32 parameters 184 us = 5.8 TB/s (a copy of 2 GiB reaches 4.9 TB/s there), 3001 x 1155
+// float32 7.7 us, one row of 4096 bf16 2.5 us (an empty kernel takes 1.3).  The variance is the mean of squared
+// differences from the mean, not of squares: rows with a large mean lose nothing.  Outputs are stored past the caches,
+// and inputs read past them where they cannot be there (past_caches): 203 -> 187 us.
 #include <algorithm>
 
 #include "device/rows.h"
@@ -9,7 +15,9 @@ namespace {
 
 // LANES threads hold a row in registers, VPT slots of 16 bytes each: the row is read once, the mean and then the mean
 // square of the differences come from the registers, and the next row is on its way meanwhile.  A workgroup keeps its
-// weights in registers for all its rows.
+// weights in registers for all its rows (from the caches for each row instead: 193 -> 236 us at 32768 x 8192).  The lanes
+// to a row were chosen at 1 GiB of rows: 8192 columns 256 lanes x 4 slots 176-188 us, 512 x 2 189, 1024 x 1 205; 4096
+// columns 128 x 4 180, 256 x 2 187-197, 512 x 1 205.
 template <class T, class P, int VEC, int VPT, int LANES, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_args a, bool stream) {
   constexpr int GROUPS = BLOCK / LANES, WAVES = LANES > 64 ? LANES / 64 : 1;
@@ -168,7 +176,8 @@ hipError_t norm_rows(const hf_layer_norm_args &a, int cus, hipStream_t s) {
   const int64_t sets = (a.rows + GROUPS - 1) / GROUPS, most = (int64_t)cus * kPerCu;
   const int64_t trips = (sets + most - 1) / most;
   const unsigned grid = (unsigned)((sets + trips - 1) / trips);   // every workgroup makes `trips` trips, or one less
-  hipLaunchKernelGGL((layer_norm_rows_kernel<T, P, VEC, VPT, LANES, BLOCK>), dim3(grid), dim3(BLOCK), 0, s, a, past_caches((size_t)a.rows * (size_t)a.cols * sizeof(T)));
+  hipLaunchKernelGGL((layer_norm_rows_kernel<T, P, VEC, VPT, LANES, BLOCK>), dim3(grid), dim3(BLOCK), 0, s, a,
+                     past_caches((size_t)a.rows * (size_t)a.cols * sizeof(T)));
   return hipGetLastError();
 }
 

@@ -1,4 +1,10 @@
-// The gradient of layer norm.
+// The gradient of layer norm: with h = (x - mean) rstd and g = dy w,
+//   dx = rstd (g - mean(g) - h mean(g h)),  dweight = sum over rows of dy h,  dbias = sum over rows of dy.
+//
+// Bound by HBM: x and dy are read once and dx is written once, about 14 operations an element.  Measured on an MI355X:
+// 32768 x 8192 bf16 274 us + 5 us for the sums of the parts = 5.8 TB/s, 5003 x 1155 f16 13.7 + 4.2 us, 64 x 1024 5.7 + 2.4.
+// The part draws so much power there that arithmetic costs time although it hides behind the memory: h and g formed twice
+// instead of kept in registers 320 us.
 #include <algorithm>
 
 #include "device/rows.h"
@@ -10,7 +16,8 @@ namespace {
 // One pass over the rows: LANES threads hold a row of x and of dy in registers, VPT slots of 16 bytes each, form the two
 // sums over the row that dx needs, write dx, and add dy * h and dy to the 32-bit sums of their columns, which stay in
 // registers for all rows of the workgroup.  The next row is on its way meanwhile.  A workgroup leaves one row of sums for
-// dweight and one for dbias in `parts`; sum_parts_kernel adds them up in the order of the workgroups.
+// dweight and one for dbias in `parts`; sum_parts_kernel adds them up in an order of its own.  One workgroup a CU: two
+// write twice the parts and hold no more rows (150 registers a thread), 18 against 14 us at 5003 x 1155.
 template <class T, class P, int VEC, int VPT, int LANES, int BLOCK, bool PARAMS>
 __global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_backward_args a, float *parts, bool stream) {
   constexpr int GROUPS = BLOCK / LANES, WAVES = LANES > 64 ? LANES / 64 : 1;

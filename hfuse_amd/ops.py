@@ -59,7 +59,8 @@ class Op:
     args: Any
     outputs: Tuple[Any, ...]
     keep: Tuple[Any, ...] = ()
-    device: Any = None     # token-model operators: where their tensors live
+    device: Any = None     # token-model operators: where their tensors live,
+    made_on: int = 0       # and the stream that was current when they were allocated
 
 
 def im2col(x, kernel_size, dilation=1, padding=0, stride=1) -> Op:
@@ -210,7 +211,7 @@ def embedding(tokens, weight, scale: float = 1.0) -> Op:
     vocab, cols = weight.shape
     w = _as_rows(weight, cols)
     out = weight.new_empty((*tokens.shape, cols))
-    return Op("embedding_forward", H.embedding_args(tok, w, out, scale), (out,), (tok, w, out), weight.device)
+    return _token_op("embedding_forward", H.embedding_args(tok, w, out, scale), (out,), (tok, w, out), weight.device)
 
 
 def embedding_backward(dy, tokens, num_embeddings: int, scale: float = 1.0, padding_idx: Optional[int] = None,
@@ -238,7 +239,7 @@ def embedding_backward(dy, tokens, num_embeddings: int, scale: float = 1.0, padd
     g = _as_rows(dy, cols)
     out = dy.new_empty((vocab, cols), dtype=dtype)
     args = H.embedding_backward_args(g, tok, out, scale, -1 if padding_idx is None else int(padding_idx))
-    return Op("embedding_backward", args, (out,), (tok, g, out, _workspace("embedding_backward", args, dy)), dy.device)
+    return _token_op("embedding_backward", args, (out,), (tok, g, out, _workspace("embedding_backward", args, dy)), dy.device)
 
 
 def _norm_shape(x, normalized_shape, what: str) -> Tuple[int, ...]:
@@ -284,7 +285,7 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps: float = 1e-5) -
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = x.new_empty(stat, dtype=torch.float32)
     rstd = torch.empty_like(mean)
-    return Op("layer_norm_forward", H.layer_norm_args(x2, y, w, b, mean, rstd, eps, cols), (y, mean, rstd),
+    return _token_op("layer_norm_forward", H.layer_norm_args(x2, y, w, b, mean, rstd, eps, cols), (y, mean, rstd),
               (x2, w, b, y, mean, rstd), x.device)
 
 
@@ -316,7 +317,7 @@ def layer_norm_backward(dy, x, normalized_shape, mean, rstd, weight=None,
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if mask[0] else None
     dw, db = ((x.new_empty(shape) if w is None else torch.empty_like(w)) if m else None for m in mask[1:])
     args = H.layer_norm_backward_args(dy2, x2, mean, rstd, w, dx, dw, db, cols=cols)
-    return Op("layer_norm_backward", args, (dx, dw, db),
+    return _token_op("layer_norm_backward", args, (dx, dw, db),
               (dy2, x2, mean, rstd, w, dx, dw, db, _workspace("layer_norm_backward", args, x)), x.device)
 
 
@@ -385,8 +386,8 @@ def _config(cfg: Optional[H.Config]) -> H.Config:
 def run(op: Op, stream=None):
     """Launch one original kernel; returns its outputs (a tuple).
 
-    A token-model operator runs on its tensors' device, and its tensors are recorded on `stream` where that is not the
-    current stream, so that they may be dropped as soon as the call returns."""
+    A token-model operator runs on its tensors' device, and where it runs on another stream than the one that was current
+    when it was built, its tensors are recorded on that stream: they may be dropped as soon as the call returns."""
     if op.device is not None:
         return _run_on_device(op, stream)
     count = getattr(op, "count", 0)
@@ -397,17 +398,21 @@ def run(op: Op, stream=None):
     return op.outputs
 
 
+def _token_op(kernel: str, args, outputs, keep, device) -> Op:
+    return Op(kernel, args, outputs, keep, device, torch._C._cuda_getCurrentRawStream(device.index))
+
+
 def _run_on_device(op: Op, stream):
     index = op.device.index
-    if stream is None and torch.cuda.current_device() == index:
-        H.launch_native(op.kernel, op.args, stream=torch._C._cuda_getCurrentRawStream(index))   # (current_stream() without its object)
-        return op.outputs
-    current = torch.cuda.current_stream(op.device)
-    used = current if stream is None else stream if isinstance(stream, torch.cuda.Stream) else \
-        torch.cuda.ExternalStream(int(stream), device=op.device)
-    with torch.cuda.device(op.device):
-        H.launch_native(op.kernel, op.args, stream=used)
-    if used != current:
+    # (what current_stream().cuda_stream gives, without making the object)
+    raw = torch._C._cuda_getCurrentRawStream(index) if stream is None else int(getattr(stream, "cuda_stream", stream))
+    if torch.cuda.current_device() == index:
+        H.launch_native(op.kernel, op.args, stream=raw)
+    else:
+        with torch.cuda.device(op.device):
+            H.launch_native(op.kernel, op.args, stream=raw)
+    if raw != op.made_on:   # their memory must not go to someone else before this stream is done with it
+        used = torch.cuda.ExternalStream(raw, device=op.device) if raw else torch.cuda.default_stream(op.device)
         for t in op.keep:
             if t is not None:
                 t.record_stream(used)

@@ -556,12 +556,35 @@ def test_two_graphs_and_a_side_stream(cuda):
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
     s = streams[0]
     s.wait_stream(torch.cuda.current_stream())
-    got = [ops.run(ops.embedding_backward(dy[i % 2], tok[i % 2], vocab), stream=s)[0] for i in range(4)]
+    got = [ops.run(ops.embedding_backward(dy[0], tok[0], vocab), stream=0)[0]]             # the default stream by its handle
+    s.wait_stream(torch.cuda.current_stream())
+    got += [ops.run(ops.embedding_backward(dy[i % 2], tok[i % 2], vocab), stream=s)[0] for i in range(4)]
     got += [ops.run(ops.embedding_backward(dy[0], tok[0], vocab), stream=s.cuda_stream)[0]]
     filler = [torch.full((1 << 20,), 7.0, device=cuda) for _ in range(8)]                # would reuse freed workspaces
     s.synchronize()
     torch.cuda.synchronize()
-    assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got)) and len(filler) == 8
+    assert all(torch.equal(g, want[i]) for g, i in zip(got, (0, 0, 1, 0, 1, 0))) and len(filler) == 8
+
+
+def test_run_on_a_stream_that_is_late(cuda):
+    """An op built on one stream and run where another is current: its workspace is not given away before that one is done."""
+    n, vocab, cols = 30000, 3000, 256
+    tok, dy = torch.randint(0, vocab, (n,), generator=gen(90)).to(cuda), rand((n, cols), 91).to(cuda)
+    want = ops.run(ops.embedding_backward(dy, tok, vocab))[0].clone()
+    busy = torch.randn((4096, 4096), device=cuda)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    op = ops.embedding_backward(dy, tok, vocab)
+    size = op.keep[-1].numel()
+    with torch.cuda.stream(s):
+        for _ in range(20):
+            busy = torch.tanh(busy @ busy)
+        (got,) = ops.run(op)
+    del op
+    junk = [torch.full((size,), 255, device=cuda, dtype=torch.uint8) for _ in range(3)]    # runs at once, next to the busy stream
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and all((j == 255).all() for j in junk)
 
 
 def test_operators_refuse_what_does_not_fit(cuda):
