@@ -1,7 +1,7 @@
 // Layer norm over the last dimension: mean = sum(x) / n, var = sum((x - mean)^2) / n, y = (x - mean) / sqrt(var + eps) w + b.
 //
 // Bound by HBM: a row is read once and written once, about 8 operations an element (2 a byte in 16 bits).  Measured on an
-// MI355X: 32768 x 8192 bf16 with float32 parameters 184 us = 5.8 TB/s (a copy of 2 GiB reaches 4.9 TB/s there), 3001 x 1155
+// MI355X: 32768 x 8192 bf16 with float32 parameters 183 us = 5.9 TB/s (a copy of 2 GiB reaches 4.9 TB/s there), 3001 x 1155
 // float32 7.7 us, one row of 4096 bf16 2.5 us (an empty kernel takes 1.3).  The variance is the mean of squared
 // differences from the mean, not of squares: rows with a large mean lose nothing.  Outputs are stored past the caches,
 // and inputs read past them where they cannot be there (past_caches): 203 -> 187 us.
@@ -15,9 +15,8 @@ namespace {
 
 // LANES threads hold a row in registers, VPT slots of 16 bytes each: the row is read once, the mean and then the mean
 // square of the differences come from the registers, and the next row is on its way meanwhile.  A workgroup keeps its
-// weights in registers for all its rows (from the caches for each row instead: 193 -> 236 us at 32768 x 8192).  The lanes
-// to a row were chosen at 1 GiB of rows: 8192 columns 256 lanes x 4 slots 176-188 us, 512 x 2 189, 1024 x 1 205; 4096
-// columns 128 x 4 180, 256 x 2 187-197, 512 x 1 205.
+// weights in registers for its rows.  Two slots a lane: with four (half the lanes) 8192 x 4096 bf16 takes 26.4 instead of
+// 25.4 us, 65536 x 4096 177 instead of 175, with one 27.2 and 192.
 template <class T, class P, int VEC, int VPT, int LANES, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_args a, bool stream) {
   constexpr int GROUPS = BLOCK / LANES, WAVES = LANES > 64 ? LANES / 64 : 1;
@@ -166,15 +165,16 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(hf_layer_norm_arg
   }
 }
 
-// Workgroups a CU: short ones that make a trip or two keep reads and writes of different ones apart in time and are
-// faster than a few that stay (32768 x 8192 bf16: 202, 193, 188, 176 us with 8, 16, 32, 64 a CU).  With float32 weights
-// next to 16-bit rows a workgroup reads as much for its weights as for two rows: half as many (199 -> 187 us).
+// Two rows a group of lanes in turn, if every CU has eight workgroups then: the second row is on its way while the first
+// is finished, and a workgroup is gone before its reads and writes fall into step with everyone's.  (65536 x 4096 bf16, trips
+// 1 / 2 / 3 / 4: 193 / 175 / 176 / 183 us.)  Float32 parameters next to 16-bit rows are as many bytes as two rows, and a
+// workgroup of 1024 is alone on half a CU: four (195 -> 186 us at 65536 x 4096, 207 -> 185 us at 16384 x 16384).
 template <class T, class P, int VEC, int VPT, int LANES>
 hipError_t norm_rows(const hf_layer_norm_args &a, int cus, hipStream_t s) {
   constexpr int BLOCK = LANES > 256 ? LANES : 256, GROUPS = BLOCK / LANES;
-  constexpr int kPerCu = (sizeof(P) > sizeof(T) && LANES >= 256 ? 32 : 64) * 256 / BLOCK;
-  const int64_t sets = (a.rows + GROUPS - 1) / GROUPS, most = (int64_t)cus * kPerCu;
-  const int64_t trips = (sets + most - 1) / most;
+  const int64_t sets = (a.rows + GROUPS - 1) / GROUPS;
+  constexpr int64_t kTrips = sizeof(P) > sizeof(T) || LANES == 1024 ? 4 : 2;
+  const int64_t trips = std::max<int64_t>(1, std::min(kTrips, sets / (cus * 8)));
   const unsigned grid = (unsigned)((sets + trips - 1) / trips);   // every workgroup makes `trips` trips, or one less
   hipLaunchKernelGGL((layer_norm_rows_kernel<T, P, VEC, VPT, LANES, BLOCK>), dim3(grid), dim3(BLOCK), 0, s, a,
                      past_caches((size_t)a.rows * (size_t)a.cols * sizeof(T)));
@@ -190,18 +190,17 @@ hipError_t norm_forward(const hf_layer_norm_args &a, int cus, hipStream_t s) {
   if (slots <= 16) return norm_rows<T, P, VEC, 1, 16>(a, cus, s);
   if (slots <= 32) return norm_rows<T, P, VEC, 1, 32>(a, cus, s);
   if (slots <= 64) return norm_rows<T, P, VEC, 1, 64>(a, cus, s);
-  // Fewer rows than CUs: a row's latency is all there is, and one slot a thread is the shortest (us at 1 and 256 rows of
-  // bf16 against the forms below: 4096 columns 2.5 / 3.5 and 3.9 / 4.8, 1024 columns 2.4 / 2.6 and 3.3 / 3.5; from about
-  // 1000 rows on the others win: 4096 rows of 1024 columns 7.9 / 5.3).
+  // Fewer rows than CUs: a row's latency is all there is, and one slot a thread is the shortest (one row of 2048 / 4096 bf16
+  // 2.4 / 2.5 us, with two slots 2.8 / 2.7); with more rows it is slower (4096 x 1024: 7.9 us against 5.3).
   if (a.rows <= cus) {
     if (slots <= 256) return norm_rows<T, P, VEC, 1, 256>(a, cus, s);
     if (slots <= 512) return norm_rows<T, P, VEC, 1, 512>(a, cus, s);
     if (slots <= 1024) return norm_rows<T, P, VEC, 1, 1024>(a, cus, s);
   }
   if (slots <= 128) return norm_rows<T, P, VEC, 2, 64>(a, cus, s);
-  if (slots <= 256) return norm_rows<T, P, VEC, 4, 64>(a, cus, s);
-  if (slots <= 512) return norm_rows<T, P, VEC, 4, 128>(a, cus, s);
-  if (slots <= 1024) return norm_rows<T, P, VEC, 4, 256>(a, cus, s);
+  if (slots <= 256) return norm_rows<T, P, VEC, 2, 128>(a, cus, s);
+  if (slots <= 512) return norm_rows<T, P, VEC, 2, 256>(a, cus, s);
+  if (slots <= 1024) return norm_rows<T, P, VEC, 2, 512>(a, cus, s);
   if (slots <= 2048) return norm_rows<T, P, VEC, 2, 1024>(a, cus, s);
   if (slots <= 4096) return norm_rows<T, P, VEC, 4, 1024>(a, cus, s);
   const unsigned grid = (unsigned)std::min<int64_t>(a.rows, (int64_t)cus * 2);
