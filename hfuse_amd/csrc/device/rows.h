@@ -103,17 +103,17 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// Column slots of a row shared by LANES threads, VPT slots each: thread t has slots t, t + LANES, ...
-template <int VEC, int VPT, int LANES>
+// Column slots of a row shared by `lanes` threads, VPT slots each: thread t has slots t, t + lanes, ...
+template <int VEC, int VPT>
 struct RowSlots {
   int col[VPT];       // first column (threads behind the row repeat its last slot)
   int skip[VPT];      // elements of the slot that are not this thread's to count: repeats, or all VEC behind the row
   bool whole[VPT];    // wave-uniform: no lane of the wave skips anything
-  __device__ __forceinline__ RowSlots(int t, int cols) {
+  __device__ __forceinline__ RowSlots(int t, int lanes, int cols) {
     const int slots = row_slots<VEC>(cols);
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
-      const int j = t + k * LANES;
+      const int j = t + k * lanes;
       col[k] = slot_column<VEC>(min(j, slots - 1), cols);
       skip[k] = j < slots ? slot_repeats<VEC>(j, cols) : VEC;
       whole[k] = __ballot(skip[k] != 0) == 0;

@@ -10,20 +10,22 @@
 #include "device/rows.h"
 #include "launch.h"
 
+// Every product and sum as it is written: elements that two slots hold come out alike whichever stores last.
+#pragma clang fp contract(off)
+
 namespace hfuse {
 namespace {
 
-// LANES threads hold a row in registers, VPT slots of 16 bytes each: the row is read once, the mean and then the mean
+// A group of lanes holds a row in registers, VPT slots of 16 bytes each: the row is read once, the mean and then the mean
 // square of the differences come from the registers, and the next row is on its way meanwhile.  A workgroup keeps its
-// weights in registers for its rows.  Two slots a lane: with four (half the lanes) 8192 x 4096 bf16 takes 26.4 instead of
-// 25.4 us, 65536 x 4096 177 instead of 175, with one 27.2 and 192.
+// weights in registers for its rows.  LANES: lanes to a row, 0 for whole waves whose number the launch says.
 template <class T, class P, int VEC, int VPT, int LANES, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_args a, bool stream) {
-  constexpr int GROUPS = BLOCK / LANES, WAVES = LANES > 64 ? LANES / 64 : 1;
-  constexpr bool kKeep = VPT * VEC * BLOCK <= 16 * 1024;   // weights and biases fit the registers next to two rows
-  __shared__ float part[2][BLOCK / 64];
-  const int cols = (int)a.cols, t = (int)threadIdx.x % LANES, group = (int)threadIdx.x / LANES;
-  const RowSlots<VEC, VPT, LANES> map(t, cols);
+__global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_args a, int wide_lanes, bool stream) {
+  constexpr bool kKeep = VPT <= 2 || BLOCK < 1024;   // weights and biases fit the registers next to two rows
+  __shared__ float part[2][16];
+  const int lanes = LANES ? LANES : wide_lanes, groups = (int)blockDim.x / lanes;
+  const int cols = (int)a.cols, t = (int)threadIdx.x % lanes, group = (int)threadIdx.x / lanes;
+  const RowSlots<VEC, VPT> map(t, lanes, cols);
   const P *weight = static_cast<const P *>(a.weight), *bias = static_cast<const P *>(a.bias);
   auto load_params = [&](int k, vec_t<P, VEC> &w, vec_t<P, VEC> &b) {
     w = weight ? load_vec<P, VEC>(weight + map.col[k]) : (vec_t<P, VEC>)(P)1.0f;
@@ -35,15 +37,14 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_ar
     for (int k = 0; k < VPT; k++) load_params(k, w[k], b[k]);
   }
   const float inv = 1.0f / (float)cols;
-  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  const int64_t step = (int64_t)gridDim.x * groups;
   auto sum_row = [&](float v, int which) {
-    v = lanes_sum<(LANES < 64 ? LANES : 64)>(v);
-    if constexpr (LANES > 64) {
+    v = lanes_sum<(LANES ? LANES : 64)>(v);
+    if constexpr (LANES == 0) {   // the waves of the row, 16 at most
       if ((threadIdx.x & 63u) == 0) part[which][threadIdx.x >> 6] = v;
       __syncthreads();   // two slots in turn: a slot is written again only behind the other one's barrier
-      v = 0.0f;
-#pragma unroll
-      for (int i = 0; i < WAVES; i++) v += part[which][group * WAVES + i];
+      const int i = (int)threadIdx.x & 15, waves = lanes >> 6;
+      v = lanes_sum<16>(i < waves ? part[which][group * waves + i] : 0.0f);
     }
     return v;
   };
@@ -53,8 +54,8 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_ar
 #pragma unroll
     for (int k = 0; k < VPT; k++) next[k] = stream ? load_vec_stream<T, VEC>(x + map.col[k]) : load_vec<T, VEC>(x + map.col[k]);
   };
-  fetch((int64_t)blockIdx.x * GROUPS + group);
-  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < a.rows; base += step) {   // all groups of a workgroup make the same trips
+  fetch((int64_t)blockIdx.x * groups + group);
+  for (int64_t base = (int64_t)blockIdx.x * groups; base < a.rows; base += step) {   // all groups of a workgroup make the same trips
     const int64_t row = base + group;
     vec_t<T, VEC> x[VPT];
 #pragma unroll
@@ -80,13 +81,13 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_ar
       for (int e = 0; e < VEC; e++) d[k][e] = elem<T, VEC>(x[k], e) - mean;
       if (map.whole[k]) {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) s += d[k][e] * d[k][e];
+        for (int e = 0; e < VEC; e++) s = fmaf(d[k][e], d[k][e], s);
       } else {
 #pragma unroll
         for (int e = 0; e < VEC; e++) s += e >= map.skip[k] ? d[k][e] * d[k][e] : 0.0f;
       }
     }
-    const float rstd = 1.0f / sqrtf(sum_row(s, 1) * inv + a.eps);
+    const float rstd = rsqrtf(sum_row(s, 1) * inv + a.eps);
     if (row < a.rows) {
       T *y = static_cast<T *>(a.y) + row * a.y_stride;
 #pragma unroll
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_ar
         }
         float out[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) out[e] = d[k][e] * rstd * elem<P, VEC>(wk, e) + elem<P, VEC>(bk, e);
+        for (int e = 0; e < VEC; e++) out[e] = fmaf(d[k][e] * rstd, elem<P, VEC>(wk, e), elem<P, VEC>(bk, e));
         store_vec_stream<T, VEC>(y + map.col[k], round_vec<T, VEC>(out));
       }
       if (t == 0) {
@@ -143,10 +144,10 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(hf_layer_norm_arg
 #pragma unroll
       for (int e = 0; e < VEC; e++) {
         const float d = e >= skip ? elem<T, VEC>(v, e) - mean : 0.0f;
-        s += d * d;
+        s = fmaf(d, d, s);
       }
     }
-    const float rstd = 1.0f / sqrtf(sum_row(s, 1) / (float)cols + a.eps);
+    const float rstd = rsqrtf(sum_row(s, 1) / (float)cols + a.eps);
     T *y = static_cast<T *>(a.y) + row * a.y_stride;
     for (int j = tid; j < slots; j += 1024) {
       const int c = slot_column<VEC>(j, cols);
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(hf_layer_norm_arg
       const vec_t<P, VEC> b = a.bias ? load_vec<P, VEC>(static_cast<const P *>(a.bias) + c) : (vec_t<P, VEC>)(P)0.0f;
       float out[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; e++) out[e] = (elem<T, VEC>(v, e) - mean) * rstd * elem<P, VEC>(w, e) + elem<P, VEC>(b, e);
+      for (int e = 0; e < VEC; e++) out[e] = fmaf((elem<T, VEC>(v, e) - mean) * rstd, elem<P, VEC>(w, e), elem<P, VEC>(b, e));
       store_vec<T, VEC>(y + c, round_vec<T, VEC>(out));
     }
     if (tid == 0) {
@@ -169,14 +170,14 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(hf_layer_norm_arg
 // is finished, and a workgroup is gone before its reads and writes fall into step with everyone's.  (65536 x 4096 bf16, trips
 // 1 / 2 / 3 / 4: 193 / 175 / 176 / 183 us.)  Float32 parameters next to 16-bit rows are as many bytes as two rows, and a
 // workgroup of 1024 is alone on half a CU: four (195 -> 186 us at 65536 x 4096, 207 -> 185 us at 16384 x 16384).
-template <class T, class P, int VEC, int VPT, int LANES>
-hipError_t norm_rows(const hf_layer_norm_args &a, int cus, hipStream_t s) {
-  constexpr int BLOCK = LANES > 256 ? LANES : 256, GROUPS = BLOCK / LANES;
-  const int64_t sets = (a.rows + GROUPS - 1) / GROUPS;
-  constexpr int64_t kTrips = sizeof(P) > sizeof(T) || LANES == 1024 ? 4 : 2;
+template <class T, class P, int VEC, int VPT, int LANES, int BLOCK>
+hipError_t norm_rows(const hf_layer_norm_args &a, int lanes, int cus, hipStream_t s) {
+  const int groups = std::max(1, 256 / lanes);
+  const int64_t sets = (a.rows + groups - 1) / groups;
+  const int64_t kTrips = sizeof(P) > sizeof(T) || lanes > 512 ? 4 : 2;
   const int64_t trips = std::max<int64_t>(1, std::min(kTrips, sets / (cus * 8)));
   const unsigned grid = (unsigned)((sets + trips - 1) / trips);   // every workgroup makes `trips` trips, or one less
-  hipLaunchKernelGGL((layer_norm_rows_kernel<T, P, VEC, VPT, LANES, BLOCK>), dim3(grid), dim3(BLOCK), 0, s, a,
+  hipLaunchKernelGGL((layer_norm_rows_kernel<T, P, VEC, VPT, LANES, BLOCK>), dim3(grid), dim3((unsigned)(groups * lanes)), 0, s, a, lanes,
                      past_caches((size_t)a.rows * (size_t)a.cols * sizeof(T)));
   return hipGetLastError();
 }
@@ -184,25 +185,26 @@ hipError_t norm_rows(const hf_layer_norm_args &a, int cus, hipStream_t s) {
 template <class T, class P>
 hipError_t norm_forward(const hf_layer_norm_args &a, int cus, hipStream_t s) {
   constexpr int VEC = kVec<T>;
-  if (a.cols < VEC) return norm_rows<T, P, 1, 1, 8>(a, cus, s);
+  if (a.cols < VEC) return norm_rows<T, P, 1, 1, 8, 256>(a, 8, cus, s);
   const int64_t slots = (a.cols + VEC - 1) / VEC;
-  if (slots <= 8) return norm_rows<T, P, VEC, 1, 8>(a, cus, s);
-  if (slots <= 16) return norm_rows<T, P, VEC, 1, 16>(a, cus, s);
-  if (slots <= 32) return norm_rows<T, P, VEC, 1, 32>(a, cus, s);
-  if (slots <= 64) return norm_rows<T, P, VEC, 1, 64>(a, cus, s);
+  if (slots <= 8) return norm_rows<T, P, VEC, 1, 8, 256>(a, 8, cus, s);
+  if (slots <= 16) return norm_rows<T, P, VEC, 1, 16, 256>(a, 16, cus, s);
+  if (slots <= 32) return norm_rows<T, P, VEC, 1, 32, 256>(a, 32, cus, s);
+  if (slots <= 64) return norm_rows<T, P, VEC, 1, 64, 256>(a, 64, cus, s);
+  const int waves = (int)std::min<int64_t>((slots + 63) / 64, 65);   // wavefronts with one slot a lane
   // Fewer rows than CUs: a row's latency is all there is, and one slot a thread is the shortest (one row of 2048 / 4096 bf16
   // 2.4 / 2.5 us, with two slots 2.8 / 2.7); with more rows it is slower (4096 x 1024: 7.9 us against 5.3).
-  if (a.rows <= cus) {
-    if (slots <= 256) return norm_rows<T, P, VEC, 1, 256>(a, cus, s);
-    if (slots <= 512) return norm_rows<T, P, VEC, 1, 512>(a, cus, s);
-    if (slots <= 1024) return norm_rows<T, P, VEC, 1, 1024>(a, cus, s);
-  }
-  if (slots <= 128) return norm_rows<T, P, VEC, 2, 64>(a, cus, s);
-  if (slots <= 256) return norm_rows<T, P, VEC, 2, 128>(a, cus, s);
-  if (slots <= 512) return norm_rows<T, P, VEC, 2, 256>(a, cus, s);
-  if (slots <= 1024) return norm_rows<T, P, VEC, 2, 512>(a, cus, s);
-  if (slots <= 2048) return norm_rows<T, P, VEC, 2, 1024>(a, cus, s);
-  if (slots <= 4096) return norm_rows<T, P, VEC, 4, 1024>(a, cus, s);
+  if (a.rows <= cus && waves <= 16) return norm_rows<T, P, VEC, 1, 0, 1024>(a, waves * 64, cus, s);
+  // Two slots a lane (with four 8192 x 4096 bf16 takes 26.4 instead of 25.4 us, 65536 x 4096 177 instead of 175; with one
+  // 27.2 and 192), one or three where that leaves fewer lanes without a slot: their arithmetic costs the same.
+  if (waves == 2) return norm_rows<T, P, VEC, 2, 64, 256>(a, 64, cus, s);
+  if (waves == 3) return norm_rows<T, P, VEC, 3, 64, 256>(a, 64, cus, s);
+  if (waves <= 16 && waves % 2 && waves % 3 == 0) return norm_rows<T, P, VEC, 3, 0, 512>(a, waves / 3 * 64, cus, s);
+  if (waves < 8 && waves % 2) return norm_rows<T, P, VEC, 1, 0, 1024>(a, waves * 64, cus, s);
+  if (waves <= 16) return norm_rows<T, P, VEC, 2, 0, 512>(a, (waves + 1) / 2 * 64, cus, s);
+  if (waves <= 32) return norm_rows<T, P, VEC, 2, 0, 1024>(a, (waves + 1) / 2 * 64, cus, s);
+  if (waves <= 48) return norm_rows<T, P, VEC, 3, 0, 1024>(a, (waves + 2) / 3 * 64, cus, s);
+  if (waves <= 64) return norm_rows<T, P, VEC, 4, 0, 1024>(a, (waves + 3) / 4 * 64, cus, s);
   const unsigned grid = (unsigned)std::min<int64_t>(a.rows, (int64_t)cus * 2);
   hipLaunchKernelGGL((layer_norm_long_kernel<T, P>), dim3(grid), dim3(1024), 0, s, a);
   return hipGetLastError();

@@ -10,23 +10,27 @@
 #include "device/rows.h"
 #include "launch.h"
 
+// Every product and sum as it is written: elements that two slots hold come out alike whichever stores last.
+#pragma clang fp contract(off)
+
 namespace hfuse {
 namespace {
 
-// One pass over the rows: LANES threads hold a row of x and of dy in registers, VPT slots of 16 bytes each, form the two
-// sums over the row that dx needs, write dx, and add dy * h and dy to the 32-bit sums of their columns, which stay in
-// registers for all rows of the workgroup.  The next row is on its way meanwhile.  A workgroup leaves one row of sums for
+// One pass over the rows: a group of lanes holds a row of x and of dy in registers, VPT slots of 16 bytes each, forms the
+// two sums over the row that dx needs, writes dx, and adds dy * h and dy to the 32-bit sums of its columns, which stay in
+// registers for all rows of the group.  The next row is on its way meanwhile.  A workgroup leaves one row of sums for
 // dweight and one for dbias in `parts`; sum_parts_kernel adds them up in an order of its own.  One workgroup a CU: two
-// write twice the parts and hold no more rows (150 registers a thread), 18 against 14 us at 5003 x 1155.
+// write twice the parts and hold no more rows (150 registers a thread), 18 against 14 us at 5003 x 1155.  LANES: lanes to a
+// row, 0 for whole waves whose number the launch says.
 template <class T, class P, int VEC, int VPT, int LANES, int BLOCK, bool PARAMS>
-__global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_backward_args a, float *parts, bool stream) {
-  constexpr int GROUPS = BLOCK / LANES, WAVES = LANES > 64 ? LANES / 64 : 1;
-  constexpr int SETS = BLOCK / (LANES > 64 ? LANES : 64);   // sets of threads with column sums of their own at the end
-  constexpr bool kKeep = BLOCK < 1024;   // a workgroup of 1024 has 128 registers a thread: weights from the caches, h and g computed twice
-  constexpr bool kAhead = VPT * VEC * BLOCK < 16 * 1024 || BLOCK < 1024;   // ... and a second row of the longest does not fit
-  __shared__ float2 part[2][BLOCK / 64];
-  const int cols = (int)a.cols, t = (int)threadIdx.x % LANES, group = (int)threadIdx.x / LANES;
-  const RowSlots<VEC, VPT, LANES> map(t, cols);
+__global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_backward_args a, float *parts, int wide_lanes, bool stream) {
+  constexpr bool kKeep = BLOCK < 1024 || VPT == 1;   // a workgroup of 1024 has 128 registers a thread: weights from the caches, h and g computed twice
+  constexpr bool kAhead = BLOCK < 1024 || VPT * VEC < 16;   // ... and a second row of the longest does not fit
+  constexpr bool kWide = LANES == 0 || LANES > 64;   // a row is whole waves
+  __shared__ float2 part[2][16];
+  const int lanes = LANES ? LANES : wide_lanes, groups = (int)blockDim.x / lanes;
+  const int cols = (int)a.cols, t = (int)threadIdx.x % lanes, group = (int)threadIdx.x / lanes;
+  const RowSlots<VEC, VPT> map(t, lanes, cols);
   const P *weight = static_cast<const P *>(a.weight);
   const bool want_dx = a.dx != nullptr, want_h = want_dx || a.dweight;   // dbias alone reads dy only
   auto load_weight = [&](int k) { return weight && want_dx ? load_vec<P, VEC>(weight + map.col[k]) : (vec_t<P, VEC>)(P)1.0f; };
@@ -42,7 +46,7 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_ba
     for (int e = 0; e < VEC; e++) dw[k][e] = db[k][e] = 0.0f;
 
   const float inv = 1.0f / (float)cols;
-  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  const int64_t step = (int64_t)gridDim.x * groups;
   vec_t<T, VEC> next_x[VPT], next_dy[VPT];
   float next_mean = 0.0f, next_rstd = 0.0f;
   auto fetch = [&](int64_t row) {
@@ -60,9 +64,9 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_ba
   };
 #pragma unroll
   for (int k = 0; k < VPT; k++) next_x[k] = (vec_t<T, VEC>)(T)0.0f;
-  if (kAhead) fetch((int64_t)blockIdx.x * GROUPS + group);
+  if (kAhead) fetch((int64_t)blockIdx.x * groups + group);
   int turn = 0;
-  for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < a.rows; base += step) {   // all groups of a workgroup make the same trips
+  for (int64_t base = (int64_t)blockIdx.x * groups; base < a.rows; base += step) {   // all groups of a workgroup make the same trips
     const int64_t row = base + group;
     const bool mine = row < a.rows;
     if (!kAhead) fetch(row);
@@ -89,10 +93,10 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_ba
           }
           if (whole() || e >= map.skip[k]) {
             sg += g;
-            sgh += g * h;
+            sgh = fmaf(g, h, sgh);
           }
           if (PARAMS && mine) {   // (repeated columns are summed twice, alike)
-            dw[k][e] += d * h;
+            dw[k][e] = fmaf(d, h, dw[k][e]);
             db[k][e] += d;
           }
         }
@@ -101,18 +105,15 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_ba
       else slot([] { return false; });
     }
     if (!want_dx) continue;
-    sg = lanes_sum<(LANES < 64 ? LANES : 64)>(sg);
-    sgh = lanes_sum<(LANES < 64 ? LANES : 64)>(sgh);
-    if constexpr (LANES > 64) {
+    sg = lanes_sum<(kWide ? 64 : LANES)>(sg);
+    sgh = lanes_sum<(kWide ? 64 : LANES)>(sgh);
+    if constexpr (kWide) {   // the waves of the row, 16 at most
       if ((threadIdx.x & 63u) == 0) part[turn][threadIdx.x >> 6] = make_float2(sg, sgh);
       __syncthreads();   // two slots in turn: a slot is written again only behind the other one's barrier
-      sg = sgh = 0.0f;
-#pragma unroll
-      for (int i = 0; i < WAVES; i++) {
-        const float2 v = part[turn][group * WAVES + i];
-        sg += v.x;
-        sgh += v.y;
-      }
+      const int i = (int)threadIdx.x & 15, waves = lanes >> 6;
+      const float2 v = i < waves ? part[turn][group * waves + i] : make_float2(0.0f, 0.0f);
+      sg = lanes_sum<16>(v.x);
+      sgh = lanes_sum<16>(v.y);
       turn ^= 1;
     }
     sg *= inv * rstd;
@@ -125,11 +126,11 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_ba
         float out[VEC];
         if constexpr (kKeep) {
 #pragma unroll
-          for (int e = 0; e < VEC; e++) out[e] = gs[k][e] * rstd - (sg + hs[k][e] * sgh);
+          for (int e = 0; e < VEC; e++) out[e] = fmaf(gs[k][e], rstd, -fmaf(hs[k][e], sgh, sg));
         } else {
           const vec_t<P, VEC> w = load_weight(k);
 #pragma unroll
-          for (int e = 0; e < VEC; e++) out[e] = elem<T, VEC>(dy[k], e) * elem<P, VEC>(w, e) * rstd - (sg + h_of(k, e) * sgh);
+          for (int e = 0; e < VEC; e++) out[e] = fmaf(elem<T, VEC>(dy[k], e) * elem<P, VEC>(w, e), rstd, -fmaf(h_of(k, e), sgh, sg));
         }
         store_vec_stream<T, VEC>(dx + map.col[k], round_vec<T, VEC>(out));
       }
@@ -139,9 +140,10 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_ba
   if constexpr (PARAMS) {
     const size_t width = (size_t)row_slots<VEC>(cols) * VEC;
     float *dw_part = parts + (size_t)blockIdx.x * 2 * width, *db_part = dw_part + width;
-    constexpr int SPAN = LANES > 64 ? LANES : 64;   // threads of a set
-    __shared__ float sums[SETS > 1 ? (SETS - 1) * SPAN * VEC : 1];
-    const int set = (int)threadIdx.x / SPAN, in_set = (int)threadIdx.x % SPAN;
+    // sets of threads with sums of their own: the groups, or the waves where a wave holds several
+    const int span = kWide ? lanes : 64, sets = (int)blockDim.x / span;
+    __shared__ float sums[(BLOCK - 64) * VEC];
+    const int set = (int)threadIdx.x / span, in_set = (int)threadIdx.x % span;
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
 #pragma unroll
@@ -150,22 +152,23 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_ba
 #pragma unroll
         for (int e = 0; e < VEC; e++) {
           v[e] = which ? db[k][e] : dw[k][e];
+          if constexpr (!kWide)
 #pragma unroll
-          for (int m = LANES; m < 64; m <<= 1) v[e] += __shfl_xor(v[e], m);   // the groups inside a wave
+            for (int m = LANES; m < 64; m <<= 1) v[e] += __shfl_xor(v[e], m);   // the groups inside a wave
         }
-        if constexpr (SETS > 1) {
+        if (sets > 1) {
           if (set > 0)
 #pragma unroll
-            for (int e = 0; e < VEC; e++) sums[((set - 1) * VEC + e) * SPAN + in_set] = v[e];
+            for (int e = 0; e < VEC; e++) sums[((set - 1) * VEC + e) * span + in_set] = v[e];
           __syncthreads();
           if (set == 0)
-            for (int i = 0; i < SETS - 1; i++)
+            for (int i = 0; i < sets - 1; i++)
 #pragma unroll
-              for (int e = 0; e < VEC; e++) v[e] += sums[(i * VEC + e) * SPAN + in_set];
+              for (int e = 0; e < VEC; e++) v[e] += sums[(i * VEC + e) * span + in_set];
           __syncthreads();
         }
-        if (set == 0 && in_set < LANES && map.skip[k] != VEC)
-          store_vec<float, VEC>((which ? db_part : dw_part) + (size_t)(t + k * LANES) * VEC, round_vec<float, VEC>(v));
+        if (set == 0 && in_set < lanes && map.skip[k] != VEC)
+          store_vec<float, VEC>((which ? db_part : dw_part) + (size_t)(t + k * lanes) * VEC, round_vec<float, VEC>(v));
       }
     }
   }
@@ -192,7 +195,7 @@ __global__ __launch_bounds__(1024) void layer_norm_long_dx_kernel(hf_layer_norm_
         const float g = elem<T, VEC>(dv, e) * elem<P, VEC>(wv, e);
         if (e >= skip) {
           sg += g;
-          sgh += g * ((elem<T, VEC>(xv, e) - mean) * rstd);
+          sgh = fmaf(g, (elem<T, VEC>(xv, e) - mean) * rstd, sgh);
         }
       }
     }
@@ -215,7 +218,7 @@ __global__ __launch_bounds__(1024) void layer_norm_long_dx_kernel(hf_layer_norm_
       float out[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; e++)
-        out[e] = rstd * (elem<T, VEC>(dv, e) * elem<P, VEC>(wv, e) - sg - (elem<T, VEC>(xv, e) - mean) * rstd * sgh);
+        out[e] = rstd * (elem<T, VEC>(dv, e) * elem<P, VEC>(wv, e) - fmaf((elem<T, VEC>(xv, e) - mean) * rstd, sgh, sg));
       store_vec<T, VEC>(dx + c, round_vec<T, VEC>(out));
     }
   }
@@ -260,9 +263,9 @@ __global__ __launch_bounds__(1024) void sum_parts_kernel(const float *parts, int
   }
 }
 
-// How the gradient is cut: threads to a row, slots to a thread, workgroups.
+// How the gradient is cut: lanes to a row, slots to a lane, threads of a workgroup, workgroups.
 struct GradPlan {
-  int vec, vpt, lanes, block;
+  int vec, vpt, lanes, block, bound;   // bound: the launch bound of the kernel that runs
   bool in_registers;
   unsigned grid;   // workgroups with a part of the columns' sums each
   size_t bytes;
@@ -273,14 +276,20 @@ GradPlan plan_grad(const hf_layer_norm_backward_args &a, int cus) {
   const int full = a.type == HF_F32 ? kVec<float> : kVec<bf16_t>;
   p.vec = a.cols < full ? 1 : full;
   const int64_t slots = (a.cols + p.vec - 1) / p.vec;
-  p.vpt = slots <= 64 ? 1 : a.type == HF_F32 && slots > 2048 ? 4 : 2;
-  p.lanes = 8;
-  while (p.lanes < 1024 && (int64_t)p.lanes * p.vpt < slots) p.lanes *= 2;
-  p.in_registers = (int64_t)p.lanes * p.vpt >= slots;
-  p.block = p.lanes > 512 ? 1024 : 512;
+  const int waves = (int)std::min<int64_t>((slots + 63) / 64, 65);   // wavefronts with one slot a lane
+  p.in_registers = waves <= (p.vec == 4 ? 64 : 32);
+  // Two slots a lane, one where that leaves fewer lanes without a slot (their arithmetic costs the same), more where a
+  // workgroup would not hold the row.
+  p.vpt = waves == 1 || (waves < 8 && waves % 2) ? 1 : waves <= 32 ? 2 : 4;
+  p.lanes = p.vpt == 4 ? 1024 : (waves + p.vpt - 1) / p.vpt * 64;
+  if (waves == 1)
+    for (p.lanes = 8; p.lanes < slots;) p.lanes *= 2;
+  // As many groups as 512 threads hold; up to 1024 threads with one slot a lane, and two groups of five or six waves.
+  p.bound = p.lanes <= 64 ? 512 : p.vpt == 1 || p.lanes > 768 ? 1024 : 768;
+  p.block = std::max(1, (p.vpt == 1 && p.lanes > 64 ? 1024 : p.lanes > 256 && p.lanes <= 384 ? 768 : 512) / p.lanes) * p.lanes;
   if (p.in_registers) {
-    const int64_t groups = p.block / p.lanes, sets = (a.rows + groups - 1) / groups, most = (int64_t)cus;
-    const int64_t trips = std::max<int64_t>(1, (sets + most - 1) / most);
+    const int64_t groups = p.block / p.lanes, sets = (a.rows + groups - 1) / groups;
+    const int64_t trips = std::max<int64_t>(1, (sets + cus - 1) / cus);
     p.grid = (unsigned)((sets + trips - 1) / trips);   // every workgroup makes `trips` trips, or one less
   } else {
     p.vec = 1;
@@ -291,35 +300,33 @@ GradPlan plan_grad(const hf_layer_norm_backward_args &a, int cus) {
   return p;
 }
 
-template <class T, class P, int VEC, int VPT, int LANES>
+template <class T, class P, int VEC, int VPT, int LANES, int BLOCK>
 hipError_t grad_rows(const hf_layer_norm_backward_args &a, const GradPlan &p, hipStream_t s) {
-  constexpr int BLOCK = LANES > 512 ? 1024 : 512;
   const bool stream = past_caches((size_t)a.rows * (size_t)a.cols * sizeof(T) * 2);
   if (a.dweight || a.dbias)
-    hipLaunchKernelGGL((layer_norm_grad_kernel<T, P, VEC, VPT, LANES, BLOCK, true>), dim3(p.grid), dim3(BLOCK), 0, s, a, static_cast<float *>(a.workspace), stream);
+    hipLaunchKernelGGL((layer_norm_grad_kernel<T, P, VEC, VPT, LANES, BLOCK, true>), dim3(p.grid), dim3(p.block), 0, s, a,
+                       static_cast<float *>(a.workspace), p.lanes, stream);
   else
-    hipLaunchKernelGGL((layer_norm_grad_kernel<T, P, VEC, VPT, LANES, BLOCK, false>), dim3(p.grid), dim3(BLOCK), 0, s, a, nullptr, stream);
+    hipLaunchKernelGGL((layer_norm_grad_kernel<T, P, VEC, VPT, LANES, BLOCK, false>), dim3(p.grid), dim3(p.block), 0, s, a, nullptr, p.lanes, stream);
   return hipGetLastError();
 }
 
 template <class T, class P>
 hipError_t grad_in_registers(const hf_layer_norm_backward_args &a, const GradPlan &p, hipStream_t s) {
   constexpr int VEC = kVec<T>;
-  if (p.vec == 1) return grad_rows<T, P, 1, 1, 8>(a, p, s);
-  if (p.vpt == 1) {
-    if (p.lanes == 8) return grad_rows<T, P, VEC, 1, 8>(a, p, s);
-    if (p.lanes == 16) return grad_rows<T, P, VEC, 1, 16>(a, p, s);
-    if (p.lanes == 32) return grad_rows<T, P, VEC, 1, 32>(a, p, s);
-    return grad_rows<T, P, VEC, 1, 64>(a, p, s);
+  if (p.vec == 1) return grad_rows<T, P, 1, 1, 8, 512>(a, p, s);
+  switch (p.lanes) {
+    case 8: return grad_rows<T, P, VEC, 1, 8, 512>(a, p, s);
+    case 16: return grad_rows<T, P, VEC, 1, 16, 512>(a, p, s);
+    case 32: return grad_rows<T, P, VEC, 1, 32, 512>(a, p, s);
+    case 64: return p.vpt == 1 ? grad_rows<T, P, VEC, 1, 64, 512>(a, p, s) : grad_rows<T, P, VEC, 2, 64, 512>(a, p, s);
   }
-  if constexpr (VEC == 4) {
-    if (p.vpt == 4) return grad_rows<T, P, VEC, 4, 1024>(a, p, s);
-  }
-  if (p.lanes == 64) return grad_rows<T, P, VEC, 2, 64>(a, p, s);
-  if (p.lanes == 128) return grad_rows<T, P, VEC, 2, 128>(a, p, s);
-  if (p.lanes == 256) return grad_rows<T, P, VEC, 2, 256>(a, p, s);
-  if (p.lanes == 512) return grad_rows<T, P, VEC, 2, 512>(a, p, s);
-  return grad_rows<T, P, VEC, 2, 1024>(a, p, s);
+  if (p.vpt == 1) return grad_rows<T, P, VEC, 1, 0, 1024>(a, p, s);
+  if (p.bound == 768) return grad_rows<T, P, VEC, 2, 0, 768>(a, p, s);
+  if (p.vpt == 2) return grad_rows<T, P, VEC, 2, 0, 1024>(a, p, s);
+  if constexpr (VEC == 4)
+    if (p.vpt == 4) return grad_rows<T, P, VEC, 4, 1024, 1024>(a, p, s);
+  return hipErrorInvalidValue;
 }
 
 template <class T, class P>

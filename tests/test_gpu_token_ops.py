@@ -497,11 +497,15 @@ def test_input_end_of_a_token_model(cuda, type):
 
 def test_same_bits_every_time(cuda):
     """Nothing depends on the order in which workgroups finish."""
-    n, vocab, cols = 20000, 5000, 136
+    same_bits(20000, 5000, 136, torch.bfloat16, cuda)
+    same_bits(5000, 900, 1155, torch.float32, cuda)      # elements that two accesses of a row hold
+    same_bits(3000, 900, 2049, torch.float16, cuda)
+
+
+def same_bits(n, vocab, cols, t, cuda):
     tok = (vocab ** torch.rand((n,), generator=gen(37))).long() - 1
-    args = [v.to(cuda) for v in (tok.clamp(0, vocab - 1), rand((vocab, cols), 38, torch.bfloat16), rand((cols,), 39, torch.bfloat16),
-                                 rand((cols,), 40, torch.bfloat16))]
-    dy = rand((n, cols), 41, torch.bfloat16).to(cuda)
+    args = [v.to(cuda) for v in (tok.clamp(0, vocab - 1), rand((vocab, cols), 38, t), rand((cols,), 39, t), rand((cols,), 40, t))]
+    dy = rand((n, cols), 41, t).to(cuda)
     first = embed_and_norm(*args, 1.5, None, dy)
     for _ in range(5):
         for a, b in zip(first, embed_and_norm(*args, 1.5, None, dy)):
