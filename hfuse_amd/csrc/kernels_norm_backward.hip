@@ -224,20 +224,33 @@ __global__ __launch_bounds__(1024) void layer_norm_long_dx_kernel(hf_layer_norm_
   }
 }
 
-// ... and the sums down the columns, a thread a column over every gridDim.y-th row.
+// ... and the sums down the columns, a thread a slot over every gridDim.y-th row.
 template <class T>
 __global__ __launch_bounds__(256) void layer_norm_long_params_kernel(hf_layer_norm_backward_args a, float *parts) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= a.cols) return;
-  float dw = 0.0f, db = 0.0f;
+  constexpr int VEC = kVec<T>;
+  const int cols = (int)a.cols, slots = row_slots<VEC>(cols), j = (int)(blockIdx.x * 256 + threadIdx.x);
+  if (j >= slots) return;
+  const int c = slot_column<VEC>(j, cols);
+  const T *x = static_cast<const T *>(a.x) + c, *dy = static_cast<const T *>(a.dy) + c;
+  float dw[VEC], db[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; e++) dw[e] = db[e] = 0.0f;
+#pragma unroll 4
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    const float d = to_f32(static_cast<const T *>(a.dy)[row * a.dy_stride + c]);
-    if (a.dweight) dw += d * ((to_f32(static_cast<const T *>(a.x)[row * a.x_stride + c]) - a.mean[row]) * a.rstd[row]);
-    db += d;
+    const vec_t<T, VEC> dv = load_vec<T, VEC>(dy + row * a.dy_stride);
+    if (a.dweight) {
+      const vec_t<T, VEC> xv = load_vec<T, VEC>(x + row * a.x_stride);
+      const float mean = a.mean[row], rstd = a.rstd[row];
+#pragma unroll
+      for (int e = 0; e < VEC; e++) dw[e] = fmaf(elem<T, VEC>(dv, e), (elem<T, VEC>(xv, e) - mean) * rstd, dw[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; e++) db[e] += elem<T, VEC>(dv, e);
   }
-  float *part = parts + (size_t)blockIdx.y * 2 * (size_t)a.cols + c;
-  part[0] = dw;
-  part[a.cols] = db;
+  const size_t width = (size_t)slots * VEC;
+  float *part = parts + (size_t)blockIdx.y * 2 * width + (size_t)j * VEC;
+  store_vec<float, VEC>(part, round_vec<float, VEC>(dw));
+  store_vec<float, VEC>(part + width, round_vec<float, VEC>(db));
 }
 
 // dweight and dbias from `nparts` rows of sums each: 64 columns a workgroup, whose sixteen waves take the rows in turn;
@@ -292,8 +305,7 @@ GradPlan plan_grad(const hf_layer_norm_backward_args &a, int cus) {
     const int64_t trips = std::max<int64_t>(1, (sets + cus - 1) / cus);
     p.grid = (unsigned)((sets + trips - 1) / trips);   // every workgroup makes `trips` trips, or one less
   } else {
-    p.vec = 1;
-    p.grid = (unsigned)std::min<int64_t>(a.rows, 64);
+    p.grid = (unsigned)std::min<int64_t>(a.rows, 128);
   }
   const size_t width = (size_t)((a.cols + p.vec - 1) / p.vec) * p.vec;
   p.bytes = a.dweight || a.dbias ? (size_t)p.grid * 2 * width * sizeof(float) : 0;
@@ -339,7 +351,7 @@ hipError_t norm_backward(const hf_layer_norm_backward_args &a, int cus, hipStrea
     if (e != hipSuccess) return e;
   } else if (a.rows > 0) {
     if (a.dx) hipLaunchKernelGGL((layer_norm_long_dx_kernel<T, P>), dim3((unsigned)std::min<int64_t>(a.rows, (int64_t)cus * 2)), dim3(1024), 0, s, a);
-    if (params) hipLaunchKernelGGL((layer_norm_long_params_kernel<T>), dim3((unsigned)((a.cols + 255) / 256), p.grid), dim3(256), 0, s, a, parts);
+    if (params) hipLaunchKernelGGL((layer_norm_long_params_kernel<T>), dim3((unsigned)((a.cols + kVec<T> * 256 - 1) / (kVec<T> * 256)), p.grid), dim3(256), 0, s, a, parts);
   }
   if (params) {
     const int64_t width = (a.cols + p.vec - 1) / p.vec * p.vec;
