@@ -1,8 +1,8 @@
 // Layer norm over the last dimension: mean = sum(x) / n, var = sum((x - mean)^2) / n, y = (x - mean) / sqrt(var + eps) w + b.
 //
 // Bound by HBM: a row is read once and written once, about 8 operations an element (2 a byte in 16 bits).  Measured on an
-// MI355X: 32768 x 8192 bf16 with float32 parameters 183 us = 5.9 TB/s (a copy of 2 GiB reaches 4.9 TB/s there), 3001 x 1155
-// float32 7.7 us, one row of 4096 bf16 2.5 us (an empty kernel takes 1.3).  The variance is the mean of squared
+// MI355X: 32768 x 8192 bf16 with float32 parameters 182 us = 5.9 TB/s (a copy of 2 GiB reaches 4.9 TB/s there), 3001 x 1155
+// float32 7.8 us, one row of 4096 bf16 2.4 us (an empty kernel takes 1.3).  The variance is the mean of squared
 // differences from the mean, not of squares: rows with a large mean lose nothing.  Outputs are stored past the caches,
 // and inputs read past them where they cannot be there (past_caches): 203 -> 187 us.
 #include <algorithm>

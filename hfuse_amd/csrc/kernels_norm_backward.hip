@@ -2,7 +2,7 @@
 //   dx = rstd (g - mean(g) - h mean(g h)),  dweight = sum over rows of dy h,  dbias = sum over rows of dy.
 //
 // Bound by HBM: x and dy are read once and dx is written once, about 14 operations an element.  Measured on an MI355X:
-// 32768 x 8192 bf16 274 us + 5 us for the sums of the parts = 5.8 TB/s, 5003 x 1155 f16 13.7 + 4.2 us, 64 x 1024 5.7 + 2.4.
+// 32768 x 8192 bf16 274 us + 5 us for the sums of the parts = 5.8 TB/s, 5003 x 1155 f16 13.0 + 4.1 us, 64 x 1024 5.9 + 2.4.
 // The part draws so much power there that arithmetic costs time although it hides behind the memory: h and g formed twice
 // instead of kept in registers 320 us.
 #include <algorithm>
