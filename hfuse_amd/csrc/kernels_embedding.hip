@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void embedding_kernel(hf_embedding_args a, int
 }
 
 // ------------------------------------------------------------------ the gradient of the table
-// The usable tokens are sorted with their positions by a stable radix sort (count_digits_kernel and place_digits_kernel
+// Few tokens take few_tokens_kernel, below.  Else the usable tokens are sorted with their positions by a stable radix sort (count_digits_kernel and place_digits_kernel
 // for each digit), the dy rows of each token are summed from the sorted list (sum_rows_kernel), and tokens whose rows were
 // shared out are joined (join_rows_kernel).  The rows of zeros -- most of the table in a small batch -- are written by
 // further workgroups of the sort's launches: a sort of some thousand tokens waits for memory most of the time on a few
@@ -278,7 +278,119 @@ __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(hf_embedding
   }
 }
 
-// Few tokens (64 WAVES KEYS at most), one launch: workgroup 0 sorts them in its LDS, digit by digit; the others have `rows`
+// As many tokens as a thread each holds kSortKeys of need no list in memory: one launch, and no workspace.  A workgroup has
+// `rows` rows of the table over one tile of columns (`lanes` slots), looks through all tokens for them, and finds none most
+// of the time: then it writes zeros.  Else it sorts the positions of its own tokens in LDS, and each group of lanes sums a
+// row of the table at a time; a token with more than kFewOwn positions is summed by all groups, joined in their order.
+// Bound by the stores of the zeros, and by the latency of launch and fetch in small tables.  Against a list sorted by one
+// workgroup, three launches in turn: 256 tokens of 32000 x 768 f32 24.9 -> 20.1 us (4.9 TB/s), 1000 of 50000 x 2048 bf16
+// 43 -> 34, of 128000 x 8192 383 -> 300 (7.0 TB/s), 1000 x 768 19 -> 12.6.  The worst case, 1024 times one token of 512
+// columns, is one CU's to read and takes 18 -> 32.
+constexpr unsigned kFewTokens = kSortStep;
+constexpr unsigned kFewRows = 256;   // one thread each
+constexpr unsigned kFewOwn = 64;
+template <class T, class O, class I, int VEC>
+__global__ __launch_bounds__(kSortThreads) void few_tokens_kernel(hf_embedding_backward_args a, unsigned rows, int row_bits, int lanes_log2,
+                                                                  unsigned tiles) {
+  __shared__ unsigned count[kSortWaves][kFewRows], start[kFewRows + 1], scan[kSortWaves];
+  __shared__ unsigned short list[kFewTokens];
+  __shared__ float sums[kSortWaves][64 * VEC];
+  const unsigned tid = threadIdx.x, wave = tid >> 6;
+  const unsigned tile = blockIdx.x % tiles, first = blockIdx.x / tiles * rows, mine = min(rows, (unsigned)a.vocab - first);
+  unsigned r[kSortKeys];
+  bool any = false;
+#pragma unroll
+  for (int u = 0; u < kSortKeys; u++) {
+    const unsigned key = list_entry<I, true>(a, nullptr, (wave * kSortKeys + u) * 64u + (tid & 63u), (unsigned)a.ntokens).y;
+    r[u] = key - first;   // (an unusable key is at least 2^31 off)
+    any |= r[u] < mine;
+  }
+  const bool present = __syncthreads_or(any);
+  if (present) {
+    for (unsigned b = tid & 63u; b < rows; b += 64) count[wave][b] = 0;   // a wave's counters are its own
+    unsigned rank[kSortKeys];
+#pragma unroll
+    for (int u = 0; u < kSortKeys; u++) rank[u] = rank_equal(r[u] & (kFewRows - 1), r[u] < mine, row_bits, tid & 63u, count[wave]);
+    __syncthreads();
+    unsigned total = 0, all;
+    if (tid < rows)
+      for (int w = 0; w < kSortWaves; w++) total += count[w][tid];
+    unsigned at = scan_block<kSortWaves>(total, scan, all) - total;
+    if (tid < rows) {
+      start[tid] = at;
+      if (tid == rows - 1) start[rows] = all;
+      for (int w = 0; w < kSortWaves; w++) {
+        const unsigned c = count[w][tid];
+        count[w][tid] = at;
+        at += c;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kSortKeys; u++)
+      if (r[u] < mine) list[count[wave][r[u]] + rank[u]] = (unsigned short)((wave * kSortKeys + u) * 64u + (tid & 63u));
+    __syncthreads();
+  }
+
+  const int lanes = 1 << lanes_log2, lane = (int)tid & (lanes - 1), cols = (int)a.cols, slots = row_slots<VEC>(cols);
+  const unsigned group = tid >> lanes_log2, groups = kSortThreads >> lanes_log2;
+  const int slot = (int)tile * lanes + lane, col = slot_column<VEC>(min(slot, slots - 1), cols);
+  const T *dy = static_cast<const T *>(a.dy) + col;
+  O *out = static_cast<O *>(a.dweight) + (size_t)first * (size_t)a.dweight_stride + col;
+  float acc[VEC];
+  auto sum = [&](unsigned from, unsigned to, unsigned step) {   // of every step-th position of the list
+    constexpr int U = 8;
+#pragma unroll
+    for (int e = 0; e < VEC; e++) acc[e] = 0.0f;
+    for (unsigned k = from; k < to; k += U * step) {
+      vec_t<T, VEC> row[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) row[u] = load_vec<T, VEC>(dy + (size_t)list[min(k + u * step, to - 1)] * (size_t)a.dy_stride);
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (k + u * step < to)
+#pragma unroll
+          for (int e = 0; e < VEC; e++) acc[e] += elem<T, VEC>(row[u], e);
+    }
+  };
+  auto put = [&](unsigned b) {
+    float v[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; e++) v[e] = acc[e] * a.scale;
+    store_vec_stream<O, VEC>(out + (size_t)b * (size_t)a.dweight_stride, round_vec<O, VEC>(v));
+  };
+  if (!present) {
+    if (slot < slots)
+      for (unsigned b = group; b < mine; b += groups) store_vec_stream<O, VEC>(out + (size_t)b * (size_t)a.dweight_stride, (vec_t<O, VEC>)(O)0.0f);
+    return;
+  }
+  for (unsigned b = group; b < mine; b += groups) {
+    if (start[b + 1] - start[b] > kFewOwn) continue;
+    sum(start[b], start[b + 1], 1);
+    if (slot < slots) put(b);
+  }
+  for (unsigned b = 0; b < mine; b++) {
+    if (start[b + 1] - start[b] <= kFewOwn) continue;
+    sum(start[b] + group, start[b + 1], groups);
+    for (int m = lanes; m < 64; m <<= 1)   // the groups of a wave
+#pragma unroll
+      for (int e = 0; e < VEC; e++) acc[e] += __shfl_xor(acc[e], m);
+#pragma unroll
+    for (int e = 0; e < VEC; e++) sums[wave][e * 64 + (int)(tid & 63u)] = acc[e];
+    __syncthreads();
+    if (group == 0 && slot < slots) {
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        acc[e] = sums[0][e * 64 + lane];
+        for (int w = 1; w < kSortWaves; w++) acc[e] += sums[w][e * 64 + lane];
+      }
+      put(b);
+    }
+    __syncthreads();   // the sums are reused by the next row
+  }
+}
+
+// Some more tokens (64 WAVES KEYS at most) next to a small table, one launch: workgroup 0 sorts them in its LDS, digit by digit; the others have `rows`
 // rows of the table each, look through the tokens themselves and write the rows of zeros.
 template <class I, int WAVES, int KEYS>
 __global__ __launch_bounds__(64 * WAVES) void sort_few_kernel(hf_embedding_backward_args a, TableScratch sc, int passes, int bits, unsigned rows,
@@ -423,8 +535,9 @@ __global__ __launch_bounds__(256) void sum_rows_kernel(hf_embedding_backward_arg
     for (int e = 0; e < VEC; e++) acc[e] += elem<T, VEC>(row, e);
   };
   // As many entries as the group has lanes at a time, one in each: a row's address is one v_readlane (a whole wave) or one
-  // shuffle away, and the tokens' last rows are the bits of one ballot.  The next U rows are on their way while U are added.
-  constexpr int U = 4;
+  // shuffle away, and the tokens' last rows are the bits of one ballot.  The next U rows are on their way while U are added
+  // (narrow rows, 4 / 8: 131072 tokens of 128 bf16 columns 75 / 71 us; wide ones: the same).
+  constexpr int U = WIDE ? 4 : 8;
   const int group_base = WIDE ? 0 : (int)(threadIdx.x & 63u) & ~(lanes - 1);
   for (unsigned base = begin; base < end; base += (unsigned)lanes) {
     const int m = (int)min((unsigned)lanes, end - base);
@@ -552,7 +665,7 @@ TablePlan plan_table(const hf_embedding_backward_args &a, int cus) {
   p.order_at = take((size_t)a.ntokens * sizeof(uint2));
   p.other_at = take(p.passes > 1 ? (size_t)a.ntokens * sizeof(uint2) : 0);
   p.partial_at = take((size_t)p.nchunks * 2 * (size_t)p.slots * (size_t)p.vec * sizeof(float));
-  p.bytes = at;
+  p.bytes = a.ntokens <= kFewTokens ? 0 : at;
   return p;
 }
 
@@ -594,8 +707,7 @@ hipError_t sort_few(const hf_embedding_backward_args &a, const TablePlan &p, con
 template <class I>
 hipError_t sort_tokens(const hf_embedding_backward_args &a, const TablePlan &p, const TableScratch &sc, const ZeroRows &all, hipStream_t s) {
   // One launch instead of two a digit: 24 against 30 us for 4096 tokens of a 2000 x 768 float32 table.  One workgroup's sort
-  // of more than 1024 tokens (11 us) is only worth it next to a small table (50000 x 2048 bf16: 54 against 52 us).
-  if (a.ntokens <= 1024) return sort_few<I, 4, 4>(a, p, sc, all, 8192, s);
+  // of 4096 tokens (11 us) is only worth it next to a small table (50000 x 2048 bf16: 54 against 52 us).
   if (a.ntokens <= 4096 && a.vocab * a.cols * (int64_t)all.element <= (int64_t)64 << 20) return sort_few<I, 8, 8>(a, p, sc, all, 65536, s);
   // the rows of zeros are shared evenly among the launches behind the first, which finds out what they are
   const unsigned parts = 2u * (unsigned)p.passes - 1u;
@@ -629,9 +741,31 @@ hipError_t sort_tokens(const hf_embedding_backward_args &a, const TablePlan &p, 
   return hipSuccess;
 }
 
+template <class T, class O, int VEC>
+hipError_t few_tokens(const hf_embedding_backward_args &a, const TablePlan &p, int cus, hipStream_t s) {
+  const int64_t row_bytes = ((int64_t)VEC * sizeof(O)) << p.lanes_log2;   // of a tile
+  // 8 KiB of the table to a workgroup (4 / 16 / 32: 52 / 38 / 45 against 34 us for 1000 tokens of 50000 x 2048 bf16); less
+  // in a small table, which would leave CUs idle (1000 x 768: 18 -> 12.6 us)
+  int64_t rows = std::max<int64_t>(1, std::min<int64_t>(kFewRows, 8192 / row_bytes));
+  while (rows > 1 && a.vocab / rows * p.col_tiles < 2 * cus) rows /= 2;
+  while (rows < kFewRows && a.vocab / rows * p.col_tiles >= 1 << 23) rows = std::min<int64_t>(rows * 2, kFewRows);   // a grid has less than 2^32 threads
+  int bits = 0;
+  while ((1 << bits) < rows) bits++;
+  const unsigned blocks = (unsigned)((a.vocab + rows - 1) / rows * p.col_tiles);
+  if (a.index_type == HF_I64)
+    hipLaunchKernelGGL((few_tokens_kernel<T, O, int64_t, VEC>), dim3(blocks), dim3(kSortThreads), 0, s, a, (unsigned)rows, bits, p.lanes_log2, p.col_tiles);
+  else
+    hipLaunchKernelGGL((few_tokens_kernel<T, O, int32_t, VEC>), dim3(blocks), dim3(kSortThreads), 0, s, a, (unsigned)rows, bits, p.lanes_log2, p.col_tiles);
+  return hipGetLastError();
+}
+
 template <class T>
 hipError_t embed_backward(const hf_embedding_backward_args &a, int cus, hipStream_t s) {
   const TablePlan p = plan_table(a, cus);
+  if (a.ntokens <= kFewTokens) {
+    if (a.out_type == HF_F32) return p.vec == 1 ? few_tokens<T, float, 1>(a, p, cus, s) : few_tokens<T, float, kVec<T>>(a, p, cus, s);
+    return p.vec == 1 ? few_tokens<T, T, 1>(a, p, cus, s) : few_tokens<T, T, kVec<T>>(a, p, cus, s);
+  }
   unsigned char *ws = static_cast<unsigned char *>(a.workspace);
   TableScratch sc;
   sc.state = reinterpret_cast<unsigned *>(ws);

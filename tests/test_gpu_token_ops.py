@@ -374,6 +374,18 @@ def test_embedding_backward_token_patterns(cuda, shape):
         check_table_grad(dy, tok, vocab, cuda, 2.0, int(tok[0]) if shape != "none" else 0, None, (shape, cols, "pad"))
 
 
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("cols", [1, 5, 24, 130, 257, 520, 1031])
+def test_embedding_backward_few_tokens_of_few_ids(cuda, type, cols):
+    """One launch's largest batch and its neighbour, an id with up to all of the rows, next to ids with one or none."""
+    t = TYPES[type]
+    for n, vocab in ((1024, 1), (1024, 3), (1025, 3), (999, 40)):
+        tok = torch.where(torch.rand((n,), generator=gen(n)) < 0.6, vocab // 2, ids(n, vocab, n))
+        for pad, dtype in ((None, None), (0, torch.float32)):
+            a = check_table_grad(rand((n, cols), n, t), tok, vocab, cuda, 1.3, pad, dtype, (type, cols, n, vocab, pad))
+            assert torch.equal(a, check_table_grad(rand((n, cols), n, t), tok, vocab, cuda, 1.3, pad, dtype))
+
+
 def test_embedding_backward_leaves_unused_rows_unread(cuda):
     """NaN in the dy rows of padding and of ids outside the table reaches nothing; other ids keep theirs to themselves."""
     n, vocab, cols = 500, 60, 72

@@ -88,12 +88,13 @@ def test_workspace_sizes():
     assert lib.hf_workspace_bytes(b"embedding_forward", C.byref(lookup()), None) == L.HF_EINVAL
     assert H.workspace_bytes("layer_norm_forward", norm()) == 0 and H.workspace_bytes("embedding_forward", lookup()) == 0
     for name, make in (("layer_norm_backward", norm_grad), ("embedding_backward", lookup_grad)):
-        need = H.workspace_bytes(name, make(workspace=None, workspace_bytes=0))
-        if need:    # too little, none at all, or off its alignment
-            for change in (dict(workspace_bytes=need - 1), dict(workspace=None), dict(workspace=8 * P + 8)):
-                with pytest.raises(hfuse_amd.HfuseError) as e:
-                    H.launch_native(name, make(**change), stream=0)
-                assert e.value.code == L.HF_EINVAL and "workspace" in e.value.message
+        size = dict(rows=4) if name == "layer_norm_backward" else dict(ntokens=5000)
+        need = H.workspace_bytes(name, make(workspace=None, workspace_bytes=0, **size))
+        assert need > 0    # too little, none at all, or off its alignment:
+        for change in (dict(workspace_bytes=need - 1), dict(workspace=None), dict(workspace=8 * P + 8)):
+            with pytest.raises(hfuse_amd.HfuseError) as e:
+                H.launch_native(name, make(**size, **change), stream=0)
+            assert e.value.code == L.HF_EINVAL and "workspace" in e.value.message
         with pytest.raises(hfuse_amd.HfuseError):
             H.workspace_bytes(name, make(cols=-1))
 
