@@ -175,7 +175,8 @@ hipError_t norm_rows(const hf_layer_norm_args &a, int lanes, int cus, hipStream_
   const int groups = std::max(1, 256 / lanes);
   const int64_t sets = (a.rows + groups - 1) / groups;
   const int64_t kTrips = sizeof(P) > sizeof(T) || lanes > 512 ? 4 : 2;
-  const int64_t trips = std::max<int64_t>(1, std::min(kTrips, sets / (cus * 8)));
+  int64_t trips = std::max<int64_t>(1, std::min(kTrips, sets / (cus * 8)));
+  while ((sets + trips - 1) / trips * (groups * lanes) >= (int64_t)1 << 32) trips *= 2;   // a grid has less than 2^32 threads
   const unsigned grid = (unsigned)((sets + trips - 1) / trips);   // every workgroup makes `trips` trips, or one less
   hipLaunchKernelGGL((layer_norm_rows_kernel<T, P, VEC, VPT, LANES, BLOCK>), dim3(grid), dim3((unsigned)(groups * lanes)), 0, s, a, lanes,
                      past_caches((size_t)a.rows * (size_t)a.cols * sizeof(T)));

@@ -456,6 +456,19 @@ def test_more_lanes_than_a_grid_has_threads(cuda):
     assert torch.equal(out[(1 << 29) - 1], w[0]) and torch.equal(out[5], w[0])
 
 
+def test_more_rows_of_layer_norm_than_a_grid_has_threads(cuda):
+    """Two rows of two elements a group of eight lanes: 2^30 rows and some are more than 2^32 lanes all the same."""
+    n = (1 << 30) + 1000
+    x = torch.zeros((n, 2), device=cuda, dtype=torch.bfloat16)
+    rows = torch.tensor([0, 5, (1 << 29) + 3, (1 << 30) - 1, 1 << 30, n - 1], device=cuda)
+    x[rows] = torch.tensor([3.0, 5.0], device=cuda, dtype=torch.bfloat16)
+    y, mean, rstd = ops.run(ops.layer_norm(x, 2, eps=0.0))
+    want = torch.tensor([-1.0, 1.0], device=cuda, dtype=torch.bfloat16).expand(len(rows), 2)
+    assert torch.equal(y[rows], want) and (mean[rows] == 4).all() and (rstd[rows] == 1).all()
+    assert int(torch.count_nonzero(mean)) == len(rows)
+    del y, mean, rstd
+
+
 def test_empty_batches(cuda):
     w = rand((9, 16), 31).to(cuda)
     none = torch.zeros((2, 0), dtype=torch.int64, device=cuda)
