@@ -218,7 +218,7 @@ def embedding_backward(dy, tokens, num_embeddings: int, scale: float = 1.0, padd
                        dtype=None) -> Op:
     """Gradient of `embedding` with respect to its weight: dy [..., D] -> [num_embeddings, D] of dy's type or float32 (`dtype`).
 
-    Row v is scale times the sum of the dy rows whose token is v, summed in 32 bits in the order of the tokens; the row of
+    Row v is scale times the sum of the dy rows whose token is v, summed in 32 bits and in one order; the row of
     `padding_idx` is zeros, and the dy rows of that token and of tokens outside [0, num_embeddings) are not read."""
     what = "embedding_backward"
     _check_typed(dy, what, "dy")

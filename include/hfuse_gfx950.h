@@ -484,9 +484,9 @@ typedef struct {
 } hf_embedding_args;
 
 /*
- * dweight row v = scale * (sum of the dy rows i with tokens[i] == v), in the order of i; zeros where no token names v and
- * for v == padding_idx (< 0: none).  All `vocab` rows are written.  The dy rows of tokens outside [0, vocab) or equal to
- * padding_idx are not read.  out_type is the type of dy or HF_F32.  workspace as for hf_layer_norm_backward_args.
+ * dweight row v = scale * (sum of the dy rows i with tokens[i] == v), added in the same order every time; zeros where no
+ * token names v and for v == padding_idx (< 0: none).  All `vocab` rows are written.  The dy rows of tokens outside
+ * [0, vocab) or equal to padding_idx are not read.  out_type is the type of dy or HF_F32.  workspace as for hf_layer_norm_backward_args.
  */
 typedef struct {
   const void *dy, *tokens;
@@ -500,7 +500,7 @@ typedef struct {
 
 /*
  * *bytes = the device memory that a native launch of this argument list needs as its `workspace` on the current device
- * (0 for kernels without one).  The sizes, types and wanted outputs are read; data and workspace pointers may be NULL,
+ * (0 if it needs none).  The sizes, types and wanted outputs are read; data and workspace pointers may be NULL,
  * except that an output left NULL counts as not wanted.
  */
 HF_API int hf_workspace_bytes(const char *kernel_name, const void *args, size_t *bytes);
