@@ -486,7 +486,8 @@ typedef struct {
 /*
  * dweight row v = scale * (sum of the dy rows i with tokens[i] == v), added in the same order every time; zeros where no
  * token names v and for v == padding_idx (< 0: none).  All `vocab` rows are written.  The dy rows of tokens outside
- * [0, vocab) or equal to padding_idx are not read.  out_type is the type of dy or HF_F32.  workspace as for hf_layer_norm_backward_args.
+ * [0, vocab) or equal to padding_idx are not read.  out_type is the type of dy or HF_F32.  workspace as for
+ * hf_layer_norm_backward_args.
  */
 typedef struct {
   const void *dy, *tokens;
