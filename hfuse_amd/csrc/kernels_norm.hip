@@ -3,9 +3,11 @@
 // Bound by HBM: a row is read once and written once, about 8 operations an element (2 a byte in 16 bits).  Measured on an
 // MI355X: 32768 x 8192 bf16 with float32 parameters 182 us = 5.9 TB/s (a copy of 2 GiB reaches 4.9 TB/s there), 3001 x 1155
 // float32 7.8 us, one row of 4096 bf16 2.4 us (an empty kernel takes 1.3).  The variance is the mean of squared
-// differences from the mean, not of squares: rows with a large mean lose nothing.  Outputs are stored past the caches,
-// and inputs read past them where they cannot be there (past_caches): 203 -> 187 us.
+// differences from the mean, not of squares, and where a row's sum is not exact the mean of the differences corrects both
+// (centred): rows with a large mean lose nothing.  Outputs are stored past the caches, and inputs read past
+// them where they cannot be there (past_caches): 203 -> 187 us.
 #include <algorithm>
+#include <type_traits>
 
 #include "device/rows.h"
 #include "launch.h"
@@ -16,13 +18,40 @@
 namespace hfuse {
 namespace {
 
+// s / n, rounded once, with inv = 1 / n rounded: the remainder of the first quotient is exact.  (s * inv alone misses whole
+// quotients: 1000.0f * 1000 * (1.0f / 1000) is 1000.00006, which makes -0.02 of a constant row where the variance is 0.)
+__device__ __forceinline__ float quotient(float s, float n, float inv) {
+  const float q = s * inv, better = fmaf(fmaf(-q, n, s), inv, q);
+  return fabsf(q) <= 3.402823466e38f ? better : q;   // infinities stay
+}
+
+// The sum of a row of 32-bit elements is rounded, so their differences d are taken from a number near the mean.  By how
+// much it is off is the mean of d, whose terms are as small as the row's spread: mean(x) = near + mean(d), and
+// var = mean(d^2) - mean(d)^2.  Of a constant row, d is a few units of x's last place, and their sum is exact.
+// 16-bit rows with a large mean have exact sums up to 2^16 (bf16) or 2^13 columns (f16): 8 or 11 bits an element and one for
+// every doubling make 24.  Their mean is rounded once, 2^-16 or 2^-13 of the elements' own step, and nothing is
+// corrected: the two operations an element would cost 184 -> 197 us at 32768 x 8192.
+struct Centre {
+  float shift, rstd;   // d - shift: the difference from the mean
+};
+__device__ __forceinline__ Centre centred(float sum_d, float sum_d2, float n, float inv, float eps) {
+  Centre c;
+  c.shift = quotient(sum_d, n, inv);
+  if (!(fabsf(c.shift) <= 3.402823466e38f)) c.shift = 0.0f;   // rows of infinities or NaN, or out of range: as they come
+  const float var = fmaf(-c.shift, c.shift, sum_d2 * inv);
+  c.rstd = rsqrtf((var < 0.0f ? 0.0f : var) + eps);           // (a NaN stays)
+  return c;
+}
+
 // A group of lanes holds a row in registers, VPT slots of 16 bytes each: the row is read once, the mean and then the mean
 // square of the differences come from the registers, and the next row is on its way meanwhile.  A workgroup keeps its
 // weights in registers for its rows.  LANES: lanes to a row, 0 for whole waves whose number the launch says.
 template <class T, class P, int VEC, int VPT, int LANES, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_args a, int wide_lanes, bool stream) {
   constexpr bool kKeep = VPT <= 2 || BLOCK < 1024;   // weights and biases fit the registers next to two rows
-  __shared__ float part[2][16];
+  // 32-bit rows, and f16 rows of more than 2^13 columns (two slots or more of 1024 threads)
+  constexpr bool kCentre = sizeof(T) == 4 || (std::is_same<T, f16_t>::value && VPT > 1 && BLOCK == 1024);
+  __shared__ float part[3][16];
   const int lanes = LANES ? LANES : wide_lanes, groups = (int)blockDim.x / lanes;
   const int cols = (int)a.cols, t = (int)threadIdx.x % lanes, group = (int)threadIdx.x / lanes;
   const RowSlots<VEC, VPT> map(t, lanes, cols);
@@ -36,13 +65,17 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_ar
 #pragma unroll
     for (int k = 0; k < VPT; k++) load_params(k, w[k], b[k]);
   }
-  const float inv = 1.0f / (float)cols;
+  const float n = (float)cols, inv = 1.0f / n;
   const int64_t step = (int64_t)gridDim.x * groups;
-  auto sum_row = [&](float v, int which) {
+  // Sums over a row.  The waves of a wide one, 16 at most, meet in LDS around a barrier: a slot is written again only behind
+  // the barrier of another.
+  auto leave = [&](float v, int which) {
     v = lanes_sum<(LANES ? LANES : 64)>(v);
-    if constexpr (LANES == 0) {   // the waves of the row, 16 at most
-      if ((threadIdx.x & 63u) == 0) part[which][threadIdx.x >> 6] = v;
-      __syncthreads();   // two slots in turn: a slot is written again only behind the other one's barrier
+    if (LANES == 0 && (threadIdx.x & 63u) == 0) part[which][threadIdx.x >> 6] = v;
+    return v;
+  };
+  auto joined = [&](float v, int which) {
+    if constexpr (LANES == 0) {
       const int i = (int)threadIdx.x & 15, waves = lanes >> 6;
       v = lanes_sum<16>(i < waves ? part[which][group * waves + i] : 0.0f);
     }
@@ -72,22 +105,37 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_ar
         for (int e = 0; e < VEC; e++) s += e >= map.skip[k] ? elem<T, VEC>(x[k], e) : 0.0f;
       }
     }
-    const float mean = sum_row(s, 0) * inv;
+    s = leave(s, 0);
+    if constexpr (LANES == 0) __syncthreads();
+    const float near = quotient(joined(s, 0), n, inv);
     s = 0.0f;
-    float d[VPT][VEC];
+    float s2 = 0.0f, d[VPT][VEC];
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
 #pragma unroll
-      for (int e = 0; e < VEC; e++) d[k][e] = elem<T, VEC>(x[k], e) - mean;
+      for (int e = 0; e < VEC; e++) d[k][e] = elem<T, VEC>(x[k], e) - near;
       if (map.whole[k]) {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) s = fmaf(d[k][e], d[k][e], s);
+        for (int e = 0; e < VEC; e++) {
+          if constexpr (kCentre) s += d[k][e];
+          s2 = fmaf(d[k][e], d[k][e], s2);
+        }
       } else {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) s += e >= map.skip[k] ? d[k][e] * d[k][e] : 0.0f;
+        for (int e = 0; e < VEC; e++) {
+          const float counted = e >= map.skip[k] ? d[k][e] : 0.0f;
+          if constexpr (kCentre) s += counted;
+          s2 = fmaf(counted, counted, s2);
+        }
       }
     }
-    const float rstd = rsqrtf(sum_row(s, 1) * inv + a.eps);
+    s2 = leave(s2, 1);
+    if constexpr (kCentre) s = leave(s, 2);
+    if constexpr (LANES == 0) __syncthreads();
+    s2 = joined(s2, 1);
+    Centre c = {0.0f, 0.0f};
+    if constexpr (kCentre) c = centred(joined(s, 2), s2, n, inv, a.eps);
+    else c.rstd = rsqrtf(s2 * inv + a.eps);
     if (row < a.rows) {
       T *y = static_cast<T *>(a.y) + row * a.y_stride;
 #pragma unroll
@@ -102,12 +150,12 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_ar
         }
         float out[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) out[e] = fmaf(d[k][e] * rstd, elem<P, VEC>(wk, e), elem<P, VEC>(bk, e));
+        for (int e = 0; e < VEC; e++) out[e] = fmaf((kCentre ? d[k][e] - c.shift : d[k][e]) * c.rstd, elem<P, VEC>(wk, e), elem<P, VEC>(bk, e));
         store_vec_stream<T, VEC>(y + map.col[k], round_vec<T, VEC>(out));
       }
       if (t == 0) {
-        if (a.mean) a.mean[row] = mean;
-        if (a.rstd) a.rstd[row] = rstd;
+        if (a.mean) a.mean[row] = kCentre ? near + c.shift : near;
+        if (a.rstd) a.rstd[row] = c.rstd;
       }
     }
   }
@@ -117,13 +165,15 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_ar
 template <class T, class P>
 __global__ __launch_bounds__(1024) void layer_norm_long_kernel(hf_layer_norm_args a) {
   constexpr int VEC = kVec<T>;
-  __shared__ float part[2][16];
+  __shared__ float part[3][16];
   const int cols = (int)a.cols, tid = (int)threadIdx.x, slots = row_slots<VEC>(cols);
-  auto sum_row = [&](float v, int which) {
+  const float n = (float)cols, inv = 1.0f / n;
+  auto leave = [&](float v, int which) {
     v = lanes_sum<64>(v);
     if ((tid & 63) == 0) part[which][tid >> 6] = v;
-    __syncthreads();
-    v = 0.0f;
+  };
+  auto sum_of = [&](int which) {   // behind a barrier; written again only behind another sum's
+    float v = 0.0f;
     for (int i = 0; i < 16; i++) v += part[which][i];
     return v;
   };
@@ -136,18 +186,25 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(hf_layer_norm_arg
 #pragma unroll
       for (int e = 0; e < VEC; e++) s += e >= skip ? elem<T, VEC>(v, e) : 0.0f;
     }
-    const float mean = sum_row(s, 0) / (float)cols;
+    leave(s, 0);
+    __syncthreads();
+    const float near = quotient(sum_of(0), n, inv);
     s = 0.0f;
+    float s2 = 0.0f;
     for (int j = tid; j < slots; j += 1024) {
       const vec_t<T, VEC> v = load_vec<T, VEC>(x + slot_column<VEC>(j, cols));
       const int skip = slot_repeats<VEC>(j, cols);
 #pragma unroll
       for (int e = 0; e < VEC; e++) {
-        const float d = e >= skip ? elem<T, VEC>(v, e) - mean : 0.0f;
-        s = fmaf(d, d, s);
+        const float d = e >= skip ? elem<T, VEC>(v, e) - near : 0.0f;
+        s += d;
+        s2 = fmaf(d, d, s2);
       }
     }
-    const float rstd = rsqrtf(sum_row(s, 1) / (float)cols + a.eps);
+    leave(s, 1);
+    leave(s2, 2);
+    __syncthreads();
+    const Centre centre = centred(sum_of(1), sum_of(2), n, inv, a.eps);
     T *y = static_cast<T *>(a.y) + row * a.y_stride;
     for (int j = tid; j < slots; j += 1024) {
       const int c = slot_column<VEC>(j, cols);
@@ -156,12 +213,12 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(hf_layer_norm_arg
       const vec_t<P, VEC> b = a.bias ? load_vec<P, VEC>(static_cast<const P *>(a.bias) + c) : (vec_t<P, VEC>)(P)0.0f;
       float out[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; e++) out[e] = fmaf((elem<T, VEC>(v, e) - mean) * rstd, elem<P, VEC>(w, e), elem<P, VEC>(b, e));
+      for (int e = 0; e < VEC; e++) out[e] = fmaf((elem<T, VEC>(v, e) - near - centre.shift) * centre.rstd, elem<P, VEC>(w, e), elem<P, VEC>(b, e));
       store_vec<T, VEC>(y + c, round_vec<T, VEC>(out));
     }
     if (tid == 0) {
-      if (a.mean) a.mean[row] = mean;
-      if (a.rstd) a.rstd[row] = rstd;
+      if (a.mean) a.mean[row] = near + centre.shift;
+      if (a.rstd) a.rstd[row] = centre.rstd;
     }
   }
 }

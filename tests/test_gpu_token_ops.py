@@ -153,6 +153,59 @@ def test_layer_norm_hard_rows(cuda):
     assert torch.isinf(rstd).all() and torch.isnan(y).all()
 
 
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("cols", [5, 100, 1000, 1155, 1920, 5001, 6656, 12290, 14336, 20001, 33000])
+def test_layer_norm_of_constant_rows_is_the_bias(cuda, type, cols):
+    """Rows of one number come out as the bias, bit for bit, and with that number as their mean.
+
+    Whole numbers up to 2^24 / cols have exact sums (multiples of 1 below 2^24), so sum / cols is the number itself, and so it
+    is for any bf16 number up to 2^16 columns and any f16 number up to 2^13 (8 and 11 bits).  Of any other number c the rounded
+    mean is k steps of c's last place off, k <= cols / 64 + 16 or, where a row is shared by more lanes, fewer; all
+    differences are then the same k steps, cols * k < 2^24 of them add up exactly, and the mean of the differences takes them
+    back to zero."""
+    t = TYPES[type]
+    b, w = rand((cols,), 1, t), rand((cols,), 2, t)
+    top = min((1 << 24) // cols, 1024 if t != torch.bfloat16 else 256)
+    whole = torch.arange(1, top + 1, dtype=torch.float32)
+    for rows in (whole, whole[-200:], -whole[:301]):
+        x = rows[:, None].to(t).expand(len(rows), cols).contiguous()
+        assert torch.equal(x[:, 0].float(), rows)
+        y, mean, rstd = run_norm(x, w, b, 1e-5, cuda)
+        assert torch.equal(mean.cpu()[:, 0], rows) and torch.equal(y.cpu(), b.expand_as(y)), (type, cols, len(rows))
+        check(rstd, torch.full((len(rows), 1), (1e-5) ** -0.5, dtype=torch.float64), 8 * U * (1e-5) ** -0.5, "rstd")
+    any_number = torch.exp(torch.rand((300,), generator=gen(cols)) * 11).to(t)               # up to 6e4
+    x = any_number[:, None].expand(300, cols).contiguous()
+    y, mean, _ = run_norm(x, w, b, 1e-5, cuda)
+    assert torch.equal(mean.cpu()[:, 0], any_number.float()) and torch.equal(y.cpu(), b.expand_as(y)), (type, cols)
+
+
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("cols", [100, 1000, 1155, 5001, 12290, 20001])
+def test_layer_norm_of_rows_with_a_large_mean(cuda, type, cols):
+    """The rounding of the row's sum, 32-bit steps of the mean, does not reach y: only those of the differences do.
+
+    The sums of the 16-bit rows are exact up to 2^13 columns (all values in [64, 128), 2^11 steps of which 2^13 are below 2^24),
+    so their mean is off by its own rounding, U |mean|, which may stay.  Else
+    near, the rounded mean, is off by tm at most (norm64).  The differences x - near are off by U each, their mean by
+    ts = (lane + 3 U)(mean|d| + tm), so a difference from the mean by td = 2 U |d| + U tm + ts.  The mean of their squares is
+    var + (near - mean)^2 with a relative (lane + 6 U), and the square taken off again is off by 2 tm ts."""
+    t, eps = TYPES[type], 1e-5
+    w, b = rand((cols,), 1, torch.float32), rand((cols,), 2, torch.float32)
+    for rows in (3, 300):
+        x = rand((rows, cols), cols + rows, t, 1.0, 2e4 if t == torch.float32 else 100.0)
+        y, mean, rstd = run_norm(x, w, b, eps, cuda)
+        wy, wm, wr, _, tm, _ = norm64(x, w, b, eps)
+        d = x.double() - wm
+        var, size, lane = (d * d).mean(1, keepdim=True), d.abs().mean(1, keepdim=True), (cols / 64 + 16) * U
+        ts = (lane + 3 * U) * (size + tm)
+        td = 2 * U * d.abs() + U * tm + ts + (0 if t == torch.float32 else U * wm.abs())
+        trstd = wr * (0.5 * ((lane + 6 * U) * (var + tm ** 2) + 2 * tm * ts) / (var + eps) + 4 * U)
+        ty = w.double().abs() * (wr * td + d.abs() * trstd) + 4 * U * ((d * wr * w).abs() + b.double().abs())
+        check(mean, wm, ts + U * (wm.abs() + ts), (type, cols, rows, "mean"))
+        check(rstd, wr, trstd, (type, cols, rows, "rstd"))
+        check(y, wy, ty + half(t) * (wy.abs() + ty) + floor(t), (type, cols, rows, "y"))
+
+
 def grad64(dy, x, mean, rstd, w):
     n, rows = x.shape[1], x.shape[0]
     dy, x, mean, rstd = dy.double(), x.double(), mean.double().view(-1, 1), rstd.double().view(-1, 1)
