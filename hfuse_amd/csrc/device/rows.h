@@ -103,6 +103,13 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
+// s / n, rounded once, with inv = 1 / n rounded: the remainder of the first quotient is exact.  (s * inv alone misses whole
+// quotients: 1000.0f * 1000 * (1.0f / 1000) is 1000.00006, which makes -0.02 of a constant row where the variance is 0.)
+__device__ __forceinline__ float quotient(float s, float n, float inv) {
+  const float q = s * inv, better = fmaf(fmaf(-q, n, s), inv, q);
+  return fabsf(q) <= 3.402823466e38f ? better : q;   // infinities stay
+}
+
 // Column slots of a row shared by `lanes` threads, VPT slots each: thread t has slots t, t + lanes, ...
 template <int VEC, int VPT>
 struct RowSlots {

@@ -18,13 +18,6 @@
 namespace hfuse {
 namespace {
 
-// s / n, rounded once, with inv = 1 / n rounded: the remainder of the first quotient is exact.  (s * inv alone misses whole
-// quotients: 1000.0f * 1000 * (1.0f / 1000) is 1000.00006, which makes -0.02 of a constant row where the variance is 0.)
-__device__ __forceinline__ float quotient(float s, float n, float inv) {
-  const float q = s * inv, better = fmaf(fmaf(-q, n, s), inv, q);
-  return fabsf(q) <= 3.402823466e38f ? better : q;   // infinities stay
-}
-
 // The sum of a row of 32-bit elements is rounded, so their differences d are taken from a number near the mean.  By how
 // much it is off is the mean of d, whose terms are as small as the row's spread: mean(x) = near + mean(d), and
 // var = mean(d^2) - mean(d)^2.  Of a constant row, d is a few units of x's last place, and their sum is exact.

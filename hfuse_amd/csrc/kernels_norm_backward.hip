@@ -45,7 +45,7 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_ba
 #pragma unroll
     for (int e = 0; e < VEC; e++) dw[k][e] = db[k][e] = 0.0f;
 
-  const float inv = 1.0f / (float)cols;
+  const float n = (float)cols, inv = 1.0f / n;
   const int64_t step = (int64_t)gridDim.x * groups;
   vec_t<T, VEC> next_x[VPT], next_dy[VPT];
   float next_mean = 0.0f, next_rstd = 0.0f;
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_ba
       sgh = lanes_sum<16>(v.y);
       turn ^= 1;
     }
-    sg *= inv * rstd;
+    sg = quotient(sg, n, inv) * rstd;   // (of a constant g, such as the gradient of a sum, nothing is left)
     sgh *= inv * rstd;
     if (mine) {
       T *dx = static_cast<T *>(a.dx) + row * a.dx_stride;

@@ -289,6 +289,21 @@ def test_layer_norm_backward_strided_rows(cuda, cols):
         check_grad(dy[:1, :1].expand(10, cols), x, mean, rstd, w, got, ("broadcast", cols, t))
 
 
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("cols", [100, 1000, 1920, 6656, 12344, 14336, 20002])
+def test_layer_norm_backward_of_a_sum(cuda, type, cols):
+    """dy of ones without a weight: g - mean(g) is nothing.  Where the h come in pairs (h, -h) beside each other, so that every
+    partial sum of g h is nothing as well, dx is zero to the bit: rstd - rstd."""
+    t = TYPES[type]
+    half_row = rand((300, cols // 2), cols, t, 2.0)
+    x = torch.stack((half_row, -half_row), 2).view(300, cols)
+    mean, rstd = torch.zeros(300), stats(x)[1]
+    for rows in (300, 7):
+        dx, _, db = run_grad(torch.ones(rows, cols, dtype=t), x[:rows], mean[:rows], rstd[:rows], None, cuda, (1, 0, 1))
+        assert not dx.any(), (type, cols, rows, float(dx.abs().max()))
+        assert (db == rows).all()      # (whole numbers up to 2^8, or 300 = 75 * 4: exact in every type)
+
+
 def test_layer_norm_gradient_against_differences(cuda):
     """d/dx, d/dw and d/db of sum(y * c) by central differences of the forward formula in 64 bits (error about h^2 and 1e-16 / h,
     far below the 32-bit bounds of the kernel, which check_grad's tolerances also cover)."""
