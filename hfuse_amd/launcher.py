@@ -375,6 +375,8 @@ def histc_args(x, out, nbins, lo, hi) -> L.HistcArgs:
 
 
 # ------------------------------------------------------------ token-model operators
+# The public builders check the tensors they are given; the ones with an underscore only fill the struct, for callers that
+# have checked them (ops).
 _TYPE_CODES: dict = {}   # torch dtype -> HF_F32 / HF_BF16 / HF_F16, HF_I32 / HF_I64 (filled on first use: torch is imported late)
 
 
@@ -384,6 +386,28 @@ def _code(t) -> int:
         _TYPE_CODES.update({torch.float32: L.HF_F32, torch.bfloat16: L.HF_BF16, torch.float16: L.HF_F16,
                             torch.int32: L.HF_I32, torch.int64: L.HF_I64})
     return _TYPE_CODES[t.dtype]
+
+
+def _check_types(what: str, rows: dict, params: dict = {}, stats: dict = {}, tokens=None):
+    """rows: of one element type, the first one's; params: of one type, that or float32; stats: float32; None passes."""
+    import torch
+    kind = next(iter(rows.values())).dtype
+    if kind not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: {next(iter(rows))} must be float32, bfloat16 or float16, got {kind}")
+    for name, t in rows.items():
+        if t is not None and t.dtype != kind:
+            raise TypeError(f"{what}: {name} must be {kind} like {next(iter(rows))}, got {t.dtype}")
+    given = [(name, t.dtype) for name, t in params.items() if t is not None]
+    for name, d in given:
+        if d not in (kind, torch.float32):
+            raise TypeError(f"{what}: {name} must be {kind} or float32, got {d}")
+        if d != given[0][1]:
+            raise TypeError(f"{what}: {given[0][0]} and {name} must be of one type, got {given[0][1]} and {d}")
+    for name, t in stats.items():
+        if t is not None and t.dtype != torch.float32:
+            raise TypeError(f"{what}: {name} must be float32, got {t.dtype}")
+    if tokens is not None and tokens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: tokens must be int32 or int64, got {tokens.dtype}")
 
 
 def _ptr(t):
@@ -401,7 +425,11 @@ def _row_stride(t, cols: int) -> int:
 
 def layer_norm_args(x, y, weight=None, bias=None, mean=None, rstd=None, eps: float = 1e-5, cols: int = 0) -> L.LayerNormArgs:
     """x, y: contiguous, or [rows, cols] with dense rows; cols: 0 = x's last dimension; mean / rstd: [rows] float32."""
-    cols = cols or x.shape[-1]
+    _check_types("layer_norm_args", dict(x=x, y=y), dict(weight=weight, bias=bias), dict(mean=mean, rstd=rstd))
+    return _layer_norm_args(x, y, weight, bias, mean, rstd, eps, cols or x.shape[-1])
+
+
+def _layer_norm_args(x, y, weight, bias, mean, rstd, eps: float, cols: int) -> L.LayerNormArgs:
     param = weight if weight is not None else bias if bias is not None else x
     return L.LayerNormArgs(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean), _ptr(rstd), x.numel() // cols, cols,
                            _row_stride(x, cols), _row_stride(y, cols), eps, _code(x), _code(param))
@@ -409,8 +437,14 @@ def layer_norm_args(x, y, weight=None, bias=None, mean=None, rstd=None, eps: flo
 
 def layer_norm_backward_args(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=None, workspace=None,
                              cols: int = 0) -> L.LayerNormBackwardArgs:
-    """dy, x, dx as x of layer_norm_args; dweight / dbias: [cols] of one type; workspace: a byte tensor of workspace_bytes()."""
-    cols = cols or x.shape[-1]
+    """dy, x, dx as x of layer_norm_args; dweight / dbias: [cols] of weight's type; workspace: a byte tensor of
+    workspace_bytes()."""
+    _check_types("layer_norm_backward_args", dict(x=x, dy=dy, dx=dx), dict(weight=weight, dweight=dweight, dbias=dbias),
+                 dict(mean=mean, rstd=rstd))
+    return _layer_norm_backward_args(dy, x, mean, rstd, weight, dx, dweight, dbias, workspace, cols or x.shape[-1])
+
+
+def _layer_norm_backward_args(dy, x, mean, rstd, weight, dx, dweight, dbias, workspace, cols: int) -> L.LayerNormBackwardArgs:
     param = weight if weight is not None else dweight if dweight is not None else dbias if dbias is not None else x
     return L.LayerNormBackwardArgs(_ptr(dy), _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight), _ptr(dbias),
                                    x.numel() // cols, cols, _row_stride(dy, cols), _row_stride(x, cols), _row_stride(dx, cols),
@@ -419,6 +453,11 @@ def layer_norm_backward_args(dy, x, mean, rstd, weight=None, dx=None, dweight=No
 
 def embedding_args(tokens, weight, out, scale: float = 1.0) -> L.EmbeddingArgs:
     """tokens: int32 / int64, contiguous; weight: [vocab, cols], rows dense; out: contiguous, or [tokens, cols] with dense rows."""
+    _check_types("embedding_args", dict(weight=weight, out=out), tokens=tokens)
+    return _embedding_args(tokens, weight, out, scale)
+
+
+def _embedding_args(tokens, weight, out, scale: float) -> L.EmbeddingArgs:
     vocab, cols = weight.shape
     return L.EmbeddingArgs(_ptr(tokens), _ptr(weight), _ptr(out), tokens.numel(), vocab, cols, _row_stride(weight, cols),
                            _row_stride(out, cols), scale, _code(weight), _code(tokens))
@@ -426,8 +465,13 @@ def embedding_args(tokens, weight, out, scale: float = 1.0) -> L.EmbeddingArgs:
 
 def embedding_backward_args(dy, tokens, dweight, scale: float = 1.0, padding_idx: int = -1,
                             workspace=None) -> L.EmbeddingBackwardArgs:
-    """dy: contiguous, or [tokens, cols] with dense rows; dweight: [vocab, cols]; padding_idx < 0: none; workspace: a byte
-    tensor of workspace_bytes()."""
+    """dy: contiguous, or [tokens, cols] with dense rows; dweight: [vocab, cols] of dy's type or float32; padding_idx < 0:
+    none; workspace: a byte tensor of workspace_bytes()."""
+    _check_types("embedding_backward_args", dict(dy=dy), dict(dweight=dweight), tokens=tokens)
+    return _embedding_backward_args(dy, tokens, dweight, scale, padding_idx, workspace)
+
+
+def _embedding_backward_args(dy, tokens, dweight, scale: float, padding_idx: int, workspace) -> L.EmbeddingBackwardArgs:
     vocab, cols = dweight.shape
     return L.EmbeddingBackwardArgs(_ptr(dy), _ptr(tokens), _ptr(dweight), tokens.numel(), vocab, cols, _row_stride(dy, cols),
                                    _row_stride(dweight, cols), padding_idx, scale, _code(dy), _code(dweight), _code(tokens),

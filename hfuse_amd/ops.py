@@ -211,7 +211,7 @@ def embedding(tokens, weight, scale: float = 1.0) -> Op:
     vocab, cols = weight.shape
     w = _as_rows(weight, cols)
     out = weight.new_empty((*tokens.shape, cols))
-    return _token_op("embedding_forward", H.embedding_args(tok, w, out, scale), (out,), (tok, w, out), weight.device)
+    return _token_op("embedding_forward", H._embedding_args(tok, w, out, scale), (out,), (tok, w, out), weight.device)
 
 
 def embedding_backward(dy, tokens, num_embeddings: int, scale: float = 1.0, padding_idx: Optional[int] = None,
@@ -238,7 +238,7 @@ def embedding_backward(dy, tokens, num_embeddings: int, scale: float = 1.0, padd
     cols = dy.shape[-1]
     g = _as_rows(dy, cols)
     out = dy.new_empty((vocab, cols), dtype=dtype)
-    args = H.embedding_backward_args(g, tok, out, scale, -1 if padding_idx is None else int(padding_idx))
+    args = H._embedding_backward_args(g, tok, out, scale, -1 if padding_idx is None else int(padding_idx), None)
     return _token_op("embedding_backward", args, (out,), (tok, g, out, _workspace("embedding_backward", args, dy)), dy.device)
 
 
@@ -285,7 +285,7 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps: float = 1e-5) -
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = x.new_empty(stat, dtype=torch.float32)
     rstd = torch.empty_like(mean)
-    return _token_op("layer_norm_forward", H.layer_norm_args(x2, y, w, b, mean, rstd, eps, cols), (y, mean, rstd),
+    return _token_op("layer_norm_forward", H._layer_norm_args(x2, y, w, b, mean, rstd, eps, cols), (y, mean, rstd),
               (x2, w, b, y, mean, rstd), x.device)
 
 
@@ -316,7 +316,7 @@ def layer_norm_backward(dy, x, normalized_shape, mean, rstd, weight=None,
     dy2, x2, mean, rstd = _as_rows(dy, cols), _as_rows(x, cols), mean.contiguous(), rstd.contiguous()
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if mask[0] else None
     dw, db = ((x.new_empty(shape) if w is None else torch.empty_like(w)) if m else None for m in mask[1:])
-    args = H.layer_norm_backward_args(dy2, x2, mean, rstd, w, dx, dw, db, cols=cols)
+    args = H._layer_norm_backward_args(dy2, x2, mean, rstd, w, dx, dw, db, None, cols)
     return _token_op("layer_norm_backward", args, (dx, dw, db),
               (dy2, x2, mean, rstd, w, dx, dw, db, _workspace("layer_norm_backward", args, x)), x.device)
 

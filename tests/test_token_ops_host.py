@@ -132,6 +132,55 @@ def test_argument_builders_refuse_rows_that_are_not_dense():
     assert (a.rows, a.cols, a.x_stride) == (2, 18, 18)
 
 
+def rows(t=torch.float32, n=4, cols=6):
+    return torch.zeros(n, cols, dtype=t)
+
+
+HALF, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+LINE = torch.zeros(6)
+TOKENS = torch.zeros(4, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("make", [
+    lambda: H.layer_norm_args(rows(), rows(BF16)),                                       # the kernel would read or write past the end of
+    lambda: H.layer_norm_args(rows(BF16), rows(BF16), LINE, LINE.bfloat16()),            # the narrower of the two
+    lambda: H.layer_norm_args(rows(BF16), rows(BF16), None, LINE.half()),
+    lambda: H.layer_norm_args(rows(), rows(), LINE.half()),
+    lambda: H.layer_norm_args(rows(), rows(), mean=torch.zeros(4, dtype=BF16)),
+    lambda: H.layer_norm_args(rows(), rows(), rstd=torch.zeros(4, dtype=torch.float64)),
+    lambda: H.layer_norm_args(rows(torch.float64), rows(torch.float64)),
+    lambda: H.layer_norm_backward_args(rows(), rows(BF16), LINE[:4], LINE[:4]),
+    lambda: H.layer_norm_backward_args(rows(BF16), rows(BF16), LINE[:4], LINE[:4], dx=rows()),
+    lambda: H.layer_norm_backward_args(rows(BF16), rows(BF16), LINE[:4], LINE[:4], LINE, dweight=LINE.bfloat16()),
+    lambda: H.layer_norm_backward_args(rows(BF16), rows(BF16), LINE[:4], LINE[:4], None, dweight=LINE.bfloat16(), dbias=LINE),
+    lambda: H.layer_norm_backward_args(rows(), rows(), LINE[:4].half(), LINE[:4]),
+    lambda: H.embedding_args(TOKENS, rows(), rows(HALF)),
+    lambda: H.embedding_args(TOKENS.float(), rows(), rows()),
+    lambda: H.embedding_args(TOKENS.short(), rows(), rows()),
+    lambda: H.embedding_args(TOKENS, rows(torch.int32), rows(torch.int32)),
+    lambda: H.embedding_backward_args(rows(), TOKENS, rows(HALF, 9)),
+    lambda: H.embedding_backward_args(rows(), TOKENS.float(), rows(n=9)),
+])
+def test_argument_builders_refuse_mixed_types(make):
+    with pytest.raises(TypeError):
+        make()
+
+
+def test_argument_builders_take_the_types_of_the_header():
+    for t, code in ((F32, L.HF_F32), (BF16, L.HF_BF16), (HALF, L.HF_F16)):
+        for p in (t, F32):
+            pcode, line = (code if p == t else L.HF_F32), LINE.to(p)
+            a = H.layer_norm_args(rows(t), rows(t), line, line, LINE[:4], LINE[:4])
+            assert (a.type, a.param_type, a.rows, a.cols) == (code, pcode, 4, 6)
+            a = H.layer_norm_backward_args(rows(t), rows(t), LINE[:4], LINE[:4], None, rows(t), line, line)
+            assert (a.type, a.param_type) == (code, pcode)
+            for tok, icode in ((TOKENS, L.HF_I64), (TOKENS.int(), L.HF_I32)):
+                a = H.embedding_backward_args(rows(t), tok, rows(p, 9))
+                assert (a.type, a.out_type, a.index_type, a.ntokens, a.vocab) == (code, pcode, icode, 4, 9)
+                a = H.embedding_args(tok, rows(t, 9), rows(t))
+                assert (a.type, a.index_type, a.vocab) == (code, icode, 9)
+
+
 FUZZ = """
 import ctypes as C, random, sys
 ROOT = sys.argv[1]
