@@ -410,6 +410,24 @@ def _check_types(what: str, rows: dict, params: dict = {}, stats: dict = {}, tok
         raise TypeError(f"{what}: tokens must be int32 or int64, got {tokens.dtype}")
 
 
+def _check_sizes(what: str, cols: int, rows: dict, params: dict = {}, stats: dict = {}, count: int = -1):
+    """rows: all of as many rows of `cols` elements as the first one has (or `count` says); params: cols elements; stats: one
+    a row; None passes."""
+    first, t = next(iter(rows.items()))
+    if cols <= 0 or t.numel() % cols:
+        raise ValueError(f"{what}: {first} of shape {tuple(t.shape)} is not made of rows of {cols}")
+    n = t.numel() // cols if count < 0 else count
+    for group, size in ((rows, n * cols), (params, cols), (stats, n)):
+        for name, t in group.items():
+            if t is not None and t.numel() != size:
+                raise ValueError(f"{what}: {name} must hold {size} elements, got the shape {tuple(t.shape)}")
+
+
+def _check_table(what: str, name: str, t):
+    if t.dim() != 2 or t.numel() == 0:
+        raise ValueError(f"{what}: {name} must be a non-empty [vocab, cols] tensor, got the shape {tuple(t.shape)}")
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -426,7 +444,9 @@ def _row_stride(t, cols: int) -> int:
 def layer_norm_args(x, y, weight=None, bias=None, mean=None, rstd=None, eps: float = 1e-5, cols: int = 0) -> L.LayerNormArgs:
     """x, y: contiguous, or [rows, cols] with dense rows; cols: 0 = x's last dimension; mean / rstd: [rows] float32."""
     _check_types("layer_norm_args", dict(x=x, y=y), dict(weight=weight, bias=bias), dict(mean=mean, rstd=rstd))
-    return _layer_norm_args(x, y, weight, bias, mean, rstd, eps, cols or x.shape[-1])
+    cols = cols or x.shape[-1]
+    _check_sizes("layer_norm_args", cols, dict(x=x, y=y), dict(weight=weight, bias=bias), dict(mean=mean, rstd=rstd))
+    return _layer_norm_args(x, y, weight, bias, mean, rstd, eps, cols)
 
 
 def _layer_norm_args(x, y, weight, bias, mean, rstd, eps: float, cols: int) -> L.LayerNormArgs:
@@ -441,7 +461,10 @@ def layer_norm_backward_args(dy, x, mean, rstd, weight=None, dx=None, dweight=No
     workspace_bytes()."""
     _check_types("layer_norm_backward_args", dict(x=x, dy=dy, dx=dx), dict(weight=weight, dweight=dweight, dbias=dbias),
                  dict(mean=mean, rstd=rstd))
-    return _layer_norm_backward_args(dy, x, mean, rstd, weight, dx, dweight, dbias, workspace, cols or x.shape[-1])
+    cols = cols or x.shape[-1]
+    _check_sizes("layer_norm_backward_args", cols, dict(x=x, dy=dy, dx=dx), dict(weight=weight, dweight=dweight, dbias=dbias),
+                 dict(mean=mean, rstd=rstd))
+    return _layer_norm_backward_args(dy, x, mean, rstd, weight, dx, dweight, dbias, workspace, cols)
 
 
 def _layer_norm_backward_args(dy, x, mean, rstd, weight, dx, dweight, dbias, workspace, cols: int) -> L.LayerNormBackwardArgs:
@@ -454,6 +477,8 @@ def _layer_norm_backward_args(dy, x, mean, rstd, weight, dx, dweight, dbias, wor
 def embedding_args(tokens, weight, out, scale: float = 1.0) -> L.EmbeddingArgs:
     """tokens: int32 / int64, contiguous; weight: [vocab, cols], rows dense; out: contiguous, or [tokens, cols] with dense rows."""
     _check_types("embedding_args", dict(weight=weight, out=out), tokens=tokens)
+    _check_table("embedding_args", "weight", weight)
+    _check_sizes("embedding_args", weight.shape[1], dict(out=out), count=tokens.numel())
     return _embedding_args(tokens, weight, out, scale)
 
 
@@ -468,6 +493,8 @@ def embedding_backward_args(dy, tokens, dweight, scale: float = 1.0, padding_idx
     """dy: contiguous, or [tokens, cols] with dense rows; dweight: [vocab, cols] of dy's type or float32; padding_idx < 0:
     none; workspace: a byte tensor of workspace_bytes()."""
     _check_types("embedding_backward_args", dict(dy=dy), dict(dweight=dweight), tokens=tokens)
+    _check_table("embedding_backward_args", "dweight", dweight)
+    _check_sizes("embedding_backward_args", dweight.shape[1], dict(dy=dy), count=tokens.numel())
     return _embedding_backward_args(dy, tokens, dweight, scale, padding_idx, workspace)
 
 

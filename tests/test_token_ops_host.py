@@ -166,6 +166,45 @@ def test_argument_builders_refuse_mixed_types(make):
         make()
 
 
+@pytest.mark.parametrize("make", [
+    lambda: H.layer_norm_args(rows(), rows(n=3)),
+    lambda: H.layer_norm_args(rows(), rows(cols=5)),
+    lambda: H.layer_norm_args(rows(), rows(), LINE[:5]),
+    lambda: H.layer_norm_args(rows(), rows(), None, torch.zeros(7)),
+    lambda: H.layer_norm_args(rows(), rows(), mean=LINE[:3]),
+    lambda: H.layer_norm_args(rows(), rows(), rstd=LINE[:5]),
+    lambda: H.layer_norm_args(rows(), rows(), cols=5),
+    lambda: H.layer_norm_args(rows(), rows(), cols=-6),
+    lambda: H.layer_norm_args(rows(cols=0), rows(cols=0)),
+    lambda: H.layer_norm_backward_args(rows(n=3), rows(), LINE[:4], LINE[:4]),
+    lambda: H.layer_norm_backward_args(rows(), rows(), LINE[:3], LINE[:4]),
+    lambda: H.layer_norm_backward_args(rows(), rows(), LINE[:4], LINE[:4], dx=rows(n=3)),
+    lambda: H.layer_norm_backward_args(rows(), rows(), LINE[:4], LINE[:4], dweight=LINE[:5]),
+    lambda: H.layer_norm_backward_args(rows(), rows(), LINE[:4], LINE[:4], dbias=torch.zeros(4, 6)),
+    lambda: H.embedding_args(TOKENS, rows(n=9), rows(n=3)),
+    lambda: H.embedding_args(TOKENS, rows(n=9), rows(cols=5)),
+    lambda: H.embedding_args(TOKENS, LINE, rows()),
+    lambda: H.embedding_args(TOKENS, rows(n=0), rows()),
+    lambda: H.embedding_backward_args(rows(n=3), TOKENS, rows(n=9)),
+    lambda: H.embedding_backward_args(rows(cols=5), TOKENS, rows(n=9)),
+    lambda: H.embedding_backward_args(rows(), TOKENS, torch.zeros(9, 2, 3)),
+])
+def test_argument_builders_refuse_sizes_that_do_not_fit(make):
+    with pytest.raises(ValueError):
+        make()
+
+
+def test_argument_builders_take_other_shapes_of_the_same_sizes():
+    a = H.layer_norm_args(torch.zeros(2, 3, 2, 9), torch.zeros(6, 18), torch.zeros(2, 9), None, torch.zeros(2, 3, 1, 1), None, cols=18)
+    assert (a.rows, a.cols) == (6, 18)
+    a = H.layer_norm_args(torch.zeros(0, 6), torch.zeros(0, 6), LINE, mean=LINE[:0])
+    assert (a.rows, a.cols) == (0, 6)
+    a = H.embedding_args(torch.zeros(2, 2, dtype=torch.int32), rows(n=9), torch.zeros(2, 2, 6))
+    assert (a.ntokens, a.cols) == (4, 6)
+    a = H.embedding_backward_args(torch.zeros(0, 6), TOKENS[:0], rows(n=9))
+    assert (a.ntokens, a.vocab) == (0, 9)
+
+
 def test_argument_builders_take_the_types_of_the_header():
     for t, code in ((F32, L.HF_F32), (BF16, L.HF_BF16), (HALF, L.HF_F16)):
         for p in (t, F32):
