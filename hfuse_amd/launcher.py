@@ -423,6 +423,16 @@ def _check_sizes(what: str, cols: int, rows: dict, params: dict = {}, stats: dic
                 raise ValueError(f"{what}: {name} must hold {size} elements, got the shape {tuple(t.shape)}")
 
 
+def _check_lines(what: str, like, tensors: dict, rows: Sequence = ()):
+    """tensors: read as adjacent elements, so contiguous; all of them and `rows` on the device of `like`; None passes."""
+    for name, t in tensors.items():
+        if t is not None and not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous")
+    for t in (*rows, *tensors.values()):
+        if t is not None and t.device != like.device:
+            raise ValueError(f"{what}: tensors on {like.device} and {t.device}")
+
+
 def _check_table(what: str, name: str, t):
     if t.dim() != 2 or t.numel() == 0:
         raise ValueError(f"{what}: {name} must be a non-empty [vocab, cols] tensor, got the shape {tuple(t.shape)}")
@@ -430,6 +440,10 @@ def _check_table(what: str, name: str, t):
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _bytes(t) -> int:
+    return 0 if t is None else t.numel() * t.element_size()
 
 
 def _row_stride(t, cols: int) -> int:
@@ -446,6 +460,7 @@ def layer_norm_args(x, y, weight=None, bias=None, mean=None, rstd=None, eps: flo
     _check_types("layer_norm_args", dict(x=x, y=y), dict(weight=weight, bias=bias), dict(mean=mean, rstd=rstd))
     cols = cols or x.shape[-1]
     _check_sizes("layer_norm_args", cols, dict(x=x, y=y), dict(weight=weight, bias=bias), dict(mean=mean, rstd=rstd))
+    _check_lines("layer_norm_args", x, dict(weight=weight, bias=bias, mean=mean, rstd=rstd), (y,))
     return _layer_norm_args(x, y, weight, bias, mean, rstd, eps, cols)
 
 
@@ -457,13 +472,15 @@ def _layer_norm_args(x, y, weight, bias, mean, rstd, eps: float, cols: int) -> L
 
 def layer_norm_backward_args(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=None, workspace=None,
                              cols: int = 0) -> L.LayerNormBackwardArgs:
-    """dy, x, dx as x of layer_norm_args; dweight / dbias: [cols] of weight's type; workspace: a byte tensor of
-    workspace_bytes()."""
+    """dy, x, dx as x of layer_norm_args; dweight / dbias: [cols] of weight's type; workspace: a tensor of
+    workspace_bytes() bytes."""
     _check_types("layer_norm_backward_args", dict(x=x, dy=dy, dx=dx), dict(weight=weight, dweight=dweight, dbias=dbias),
                  dict(mean=mean, rstd=rstd))
     cols = cols or x.shape[-1]
     _check_sizes("layer_norm_backward_args", cols, dict(x=x, dy=dy, dx=dx), dict(weight=weight, dweight=dweight, dbias=dbias),
                  dict(mean=mean, rstd=rstd))
+    _check_lines("layer_norm_backward_args", x, dict(weight=weight, dweight=dweight, dbias=dbias, mean=mean, rstd=rstd,
+                                                     workspace=workspace), (dy, dx))
     return _layer_norm_backward_args(dy, x, mean, rstd, weight, dx, dweight, dbias, workspace, cols)
 
 
@@ -471,7 +488,7 @@ def _layer_norm_backward_args(dy, x, mean, rstd, weight, dx, dweight, dbias, wor
     param = weight if weight is not None else dweight if dweight is not None else dbias if dbias is not None else x
     return L.LayerNormBackwardArgs(_ptr(dy), _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight), _ptr(dbias),
                                    x.numel() // cols, cols, _row_stride(dy, cols), _row_stride(x, cols), _row_stride(dx, cols),
-                                   _code(x), _code(param), _ptr(workspace), 0 if workspace is None else workspace.numel())
+                                   _code(x), _code(param), _ptr(workspace), _bytes(workspace))
 
 
 def embedding_args(tokens, weight, out, scale: float = 1.0) -> L.EmbeddingArgs:
@@ -479,6 +496,7 @@ def embedding_args(tokens, weight, out, scale: float = 1.0) -> L.EmbeddingArgs:
     _check_types("embedding_args", dict(weight=weight, out=out), tokens=tokens)
     _check_table("embedding_args", "weight", weight)
     _check_sizes("embedding_args", weight.shape[1], dict(out=out), count=tokens.numel())
+    _check_lines("embedding_args", weight, dict(tokens=tokens), (out,))
     return _embedding_args(tokens, weight, out, scale)
 
 
@@ -491,10 +509,11 @@ def _embedding_args(tokens, weight, out, scale: float) -> L.EmbeddingArgs:
 def embedding_backward_args(dy, tokens, dweight, scale: float = 1.0, padding_idx: int = -1,
                             workspace=None) -> L.EmbeddingBackwardArgs:
     """dy: contiguous, or [tokens, cols] with dense rows; dweight: [vocab, cols] of dy's type or float32; padding_idx < 0:
-    none; workspace: a byte tensor of workspace_bytes()."""
+    none; workspace: a tensor of workspace_bytes() bytes."""
     _check_types("embedding_backward_args", dict(dy=dy), dict(dweight=dweight), tokens=tokens)
     _check_table("embedding_backward_args", "dweight", dweight)
     _check_sizes("embedding_backward_args", dweight.shape[1], dict(dy=dy), count=tokens.numel())
+    _check_lines("embedding_backward_args", dy, dict(tokens=tokens, workspace=workspace), (dweight,))
     return _embedding_backward_args(dy, tokens, dweight, scale, padding_idx, workspace)
 
 
@@ -502,7 +521,7 @@ def _embedding_backward_args(dy, tokens, dweight, scale: float, padding_idx: int
     vocab, cols = dweight.shape
     return L.EmbeddingBackwardArgs(_ptr(dy), _ptr(tokens), _ptr(dweight), tokens.numel(), vocab, cols, _row_stride(dy, cols),
                                    _row_stride(dweight, cols), padding_idx, scale, _code(dy), _code(dweight), _code(tokens),
-                                   _ptr(workspace), 0 if workspace is None else workspace.numel())
+                                   _ptr(workspace), _bytes(workspace))
 
 
 def workspace_bytes(kernel_name: str, args) -> int:

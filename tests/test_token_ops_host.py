@@ -194,6 +194,42 @@ def test_argument_builders_refuse_sizes_that_do_not_fit(make):
         make()
 
 
+EVERY_OTHER = torch.zeros(12)[::2]
+BYTES = torch.zeros(64, dtype=torch.uint8)
+
+
+@pytest.mark.parametrize("make", [
+    lambda: H.layer_norm_args(rows(), rows(), EVERY_OTHER),
+    lambda: H.layer_norm_args(rows(), rows(), None, EVERY_OTHER),
+    lambda: H.layer_norm_args(rows(), rows(), mean=EVERY_OTHER[:4]),
+    lambda: H.layer_norm_args(rows(), rows(), rstd=torch.zeros(1).expand(4)),
+    lambda: H.layer_norm_backward_args(rows(), rows(), EVERY_OTHER[:4], LINE[:4]),
+    lambda: H.layer_norm_backward_args(rows(), rows(), LINE[:4], LINE[:4], EVERY_OTHER),
+    lambda: H.layer_norm_backward_args(rows(), rows(), LINE[:4], LINE[:4], dweight=EVERY_OTHER),
+    lambda: H.layer_norm_backward_args(rows(), rows(), LINE[:4], LINE[:4], dbias=EVERY_OTHER),
+    lambda: H.layer_norm_backward_args(rows(), rows(), LINE[:4], LINE[:4], dbias=LINE, workspace=BYTES[::2]),
+    lambda: H.embedding_args(torch.zeros(8, dtype=torch.int64)[::2], rows(n=9), rows()),
+    lambda: H.embedding_args(torch.zeros(2, 2, dtype=torch.int64).t(), rows(n=9), rows()),
+    lambda: H.embedding_backward_args(rows(), torch.zeros(8, dtype=torch.int32)[::2], rows(n=9)),
+    lambda: H.embedding_backward_args(rows(), TOKENS, rows(n=9), workspace=BYTES[::2]),
+    lambda: H.layer_norm_args(rows(), rows().to("meta")),                                # another device's memory
+    lambda: H.layer_norm_args(rows(), rows(), LINE.to("meta")),
+    lambda: H.layer_norm_backward_args(rows().to("meta"), rows(), LINE[:4], LINE[:4]),
+    lambda: H.embedding_args(TOKENS.to("meta"), rows(n=9), rows()),
+    lambda: H.embedding_backward_args(rows(), TOKENS, rows(n=9).to("meta")),
+])
+def test_argument_builders_refuse_strides_and_devices_they_would_misread(make):
+    with pytest.raises(ValueError):
+        make()
+
+
+def test_argument_builders_count_a_workspace_in_bytes():
+    for make in (lambda w: H.layer_norm_backward_args(rows(), rows(), LINE[:4], LINE[:4], dbias=LINE, workspace=w),
+                 lambda w: H.embedding_backward_args(rows(), TOKENS, rows(n=9), workspace=w)):
+        assert make(BYTES).workspace_bytes == 64 and make(BYTES).workspace == BYTES.data_ptr()
+        assert make(BYTES.view(torch.int32)).workspace_bytes == 64 and make(None).workspace_bytes == 0
+
+
 def test_argument_builders_take_other_shapes_of_the_same_sizes():
     a = H.layer_norm_args(torch.zeros(2, 3, 2, 9), torch.zeros(6, 18), torch.zeros(2, 9), None, torch.zeros(2, 3, 1, 1), None, cols=18)
     assert (a.rows, a.cols) == (6, 18)
