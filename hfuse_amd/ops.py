@@ -29,7 +29,7 @@ float16, and are launched alone:
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from numbers import Integral
 from typing import Any, Optional, Sequence, Tuple
 
@@ -59,8 +59,9 @@ class Op:
     args: Any
     outputs: Tuple[Any, ...]
     keep: Tuple[Any, ...] = ()
-    device: Any = None     # token-model operators: where their tensors live,
-    made_on: int = 0       # and the stream that was current when they were allocated
+    # (by name only: `count` of a SearchOp is the next one by position)
+    device: Any = field(default=None, kw_only=True)   # token-model operators: where their tensors live,
+    made_on: int = field(default=0, kw_only=True)     # and the stream that was current when they were allocated
 
 
 def im2col(x, kernel_size, dilation=1, padding=0, stride=1) -> Op:
@@ -399,7 +400,7 @@ def run(op: Op, stream=None):
 
 
 def _token_op(kernel: str, args, outputs, keep, device) -> Op:
-    return Op(kernel, args, outputs, keep, device, torch._C._cuda_getCurrentRawStream(device.index))
+    return Op(kernel, args, outputs, keep, device=device, made_on=torch._C._cuda_getCurrentRawStream(device.index))
 
 
 def _run_on_device(op: Op, stream):

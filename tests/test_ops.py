@@ -16,6 +16,14 @@ def test_operators_refuse_what_they_cannot_run():
             make()
 
 
+def test_search_op_takes_its_count_by_position():
+    op = ops.SearchOp("ethash_search", None, (), (), 4096)
+    assert op.count == 4096 and op.device is None
+    assert ops.Op("im2col_kernel", None, (), ("kept",)).keep == ("kept",)
+    with pytest.raises(TypeError):
+        ops.Op("im2col_kernel", None, (), (), "cuda:0")
+
+
 @pytest.mark.gpu
 def test_native_operators_match_pytorch(cuda):
     x = uniform((3, 5, 14, 18), 71)
