@@ -33,9 +33,9 @@ from dataclasses import dataclass, field
 from numbers import Integral
 from typing import Any, Optional, Sequence, Tuple
 
-import torch
-
 from . import launcher as H
+
+torch: Any = None   # imported late, as every operator does for itself: here with the first token-model operator
 
 
 def _pair(v) -> Tuple[int, int]:
@@ -152,7 +152,14 @@ def histc(x, bins: int = 100, min: float = 0.0, max: float = 0.0) -> Op:
 
 
 # ------------------------------------------------------------------ token-model operators
-_DTYPES = frozenset((torch.float32, torch.bfloat16, torch.float16))
+_DTYPES: frozenset = frozenset()   # filled with torch
+
+
+def _import_torch():
+    global torch, _DTYPES
+    import torch as module
+    _DTYPES = frozenset((module.float32, module.bfloat16, module.float16))
+    torch = module   # last: another thread may be looking
 
 
 def _check_typed(x, what: str, name: str):
@@ -203,6 +210,8 @@ def embedding(tokens, weight, scale: float = 1.0) -> Op:
     """scale * weight[tokens]: tokens [...] int32 / int64, weight [V, D] -> [..., D] of weight's type.
 
     A token outside [0, V), such as the -1 behind the last token of a padded sequence, looks up a row of zeros."""
+    if torch is None:
+        _import_torch()
     _check_typed(weight, "embedding", "weight")
     tok = _check_tokens(tokens, "embedding")
     if weight.dim() != 2 or weight.numel() == 0:
@@ -221,6 +230,8 @@ def embedding_backward(dy, tokens, num_embeddings: int, scale: float = 1.0, padd
 
     Row v is scale times the sum of the dy rows whose token is v, summed in 32 bits and in one order; the row of
     `padding_idx` is zeros, and the dy rows of that token and of tokens outside [0, num_embeddings) are not read."""
+    if torch is None:
+        _import_torch()
     what = "embedding_backward"
     _check_typed(dy, what, "dy")
     tok = _check_tokens(tokens, what)
@@ -270,6 +281,8 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps: float = 1e-5) -
     """torch.native_layer_norm: x [..., *normalized_shape] -> (y, mean, rstd), mean and rstd float32 [..., 1, ...].
 
     weight and bias are both of x's type or both float32; y is of x's type."""
+    if torch is None:
+        _import_torch()
     what = "layer_norm"
     _check_typed(x, what, "x")
     shape = _norm_shape(x, normalized_shape, what)
@@ -296,6 +309,8 @@ def layer_norm_backward(dy, x, normalized_shape, mean, rstd, weight=None,
 
     `output_mask` says which of the three are wanted, the others come back as None (default: dx, and the parameters'
     gradients where there is a weight).  dweight and dbias are of weight's type (x's without one)."""
+    if torch is None:
+        _import_torch()
     what = "layer_norm_backward"
     _check_typed(x, what, "x")
     _check_typed(dy, what, "dy")
@@ -404,6 +419,8 @@ def _token_op(kernel: str, args, outputs, keep, device) -> Op:
 
 
 def _run_on_device(op: Op, stream):
+    if torch is None:
+        _import_torch()
     index = op.device.index
     # (what current_stream().cuda_stream gives, without making the object)
     raw = torch._C._cuda_getCurrentRawStream(index) if stream is None else int(getattr(stream, "cuda_stream", stream))

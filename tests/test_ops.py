@@ -16,6 +16,16 @@ def test_operators_refuse_what_they_cannot_run():
             make()
 
 
+def test_importing_the_operators_does_not_import_torch():
+    import os
+    import subprocess
+    import sys
+    code = "import sys; import hfuse_amd.ops as o; assert 'torch' not in sys.modules; o._import_torch(); assert o.torch.float32 in o._DTYPES"
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_search_op_takes_its_count_by_position():
     op = ops.SearchOp("ethash_search", None, (), (), 4096)
     assert op.count == 4096 and op.device is None
