@@ -502,7 +502,6 @@ int prepare_blake2b(const hf_blake2b_args &a, bool sia, const SearchConstants &c
   return HF_OK;
 }
 
-// `consts`: the constants a search kernel is launched with; null = the process-wide set as it is now.
 // ------------------------------------------------ token-model operators
 constexpr int64_t kMaxCols = (int64_t)1 << 27;   // a row's bytes and the threads of a grid over it are counted in 32 bits
 bool element_type_ok(int t) { return t == HF_F32 || t == HF_BF16 || t == HF_F16; }
@@ -644,6 +643,7 @@ int launch_token_op(TokenOp op, const void *args, int grid_blocks, int block_thr
   return e == hipSuccess ? HF_OK : hip_fail(e, "native launch");
 }
 
+// `consts`: the constants a search kernel is launched with; null = the process-wide set as it is now.
 int prepare(KernelId id, const void *args, Prepared &p, const SearchConstants *consts = nullptr) {
   if (!args) return fail(HF_EINVAL, "null argument list");
   p = Prepared();
