@@ -390,11 +390,14 @@ __global__ __launch_bounds__(kSortThreads) void few_tokens_kernel(hf_embedding_b
   }
 }
 
-// Some more tokens (64 WAVES KEYS at most) next to a small table, one launch: workgroup 0 sorts them in its LDS, digit by digit; the others have `rows`
-// rows of the table each, look through the tokens themselves and write the rows of zeros.
-template <class I, int WAVES, int KEYS>
-__global__ __launch_bounds__(64 * WAVES) void sort_few_kernel(hf_embedding_backward_args a, TableScratch sc, int passes, int bits, unsigned rows,
-                                                              ZeroRows z) {
+// Some more tokens (kSortFewTokens at most) next to a small table, one launch: workgroup 0 sorts them in its LDS, digit by
+// digit; the others have `rows` rows of the table each, look through the tokens themselves and write the rows of zeros.
+constexpr int kSortFewWaves = 8, kSortFewKeys = 8;   // keys: of a thread
+constexpr int64_t kSortFewTokens = 64 * kSortFewWaves * kSortFewKeys, kSortFewBytes = 65536;   // bytes: of the table to a workgroup
+template <class I>
+__global__ __launch_bounds__(64 * kSortFewWaves) void sort_few_kernel(hf_embedding_backward_args a, TableScratch sc, int passes, int bits,
+                                                                      unsigned rows, ZeroRows z) {
+  constexpr int WAVES = kSortFewWaves, KEYS = kSortFewKeys;
   constexpr unsigned kThreads = 64 * WAVES;
   constexpr int kOwn = (kMaxBuckets + kThreads - 1) / kThreads;   // buckets of a thread
   __shared__ uint2 list[kThreads * KEYS];
@@ -629,7 +632,7 @@ struct TablePlan {
 };
 
 TablePlan plan_table(const hf_embedding_backward_args &a, int cus) {
-  TablePlan p;
+  TablePlan p = {};
   const int vec = a.type == HF_F32 ? kVec<float> : kVec<bf16_t>;
   p.vec = a.cols >= vec ? vec : 1;
   p.slots = (int)((a.cols + p.vec - 1) / p.vec);
@@ -637,6 +640,7 @@ TablePlan plan_table(const hf_embedding_backward_args &a, int cus) {
   while (p.lanes_log2 > 3 && (1 << (p.lanes_log2 - 1)) >= p.slots) p.lanes_log2--;   // (eight lanes at least: they hold the entries)
   const int lanes = 1 << p.lanes_log2;
   p.col_tiles = (unsigned)((p.slots + lanes - 1) / lanes);
+  if (a.ntokens <= kFewTokens) return p;   // few_tokens_kernel: no list, no workspace
   p.chunk = kMaxChunk;
   while (p.chunk > 8 && a.ntokens / p.chunk * p.col_tiles * lanes < (int64_t)cus * (lanes == 64 ? kWideWaves : kNarrowWaves) * 64) p.chunk /= 2;
   while (a.ntokens / p.chunk * p.col_tiles * lanes >= (int64_t)1 << 31) p.chunk *= 2;   // lanes are numbered in 32 bits
@@ -647,7 +651,7 @@ TablePlan plan_table(const hf_embedding_backward_args &a, int cus) {
   p.digit_bits = (bits + p.passes - 1) / p.passes;
   const int64_t steps = (a.ntokens + kSortStep - 1) / kSortStep;
   p.tile = (unsigned)((steps + kSortTiles - 1) / kSortTiles * kSortStep);
-  p.tiles = p.tile ? (unsigned)((a.ntokens + p.tile - 1) / p.tile) : 0;
+  p.tiles = (unsigned)((a.ntokens + p.tile - 1) / p.tile);
   const int64_t row_bytes = a.cols * (a.out_type == HF_F32 ? 4 : 2);
   p.zero_log2 = 0;   // lanes to a row of zeros: as many as it has 16-byte stores
   while (((int64_t)16 << p.zero_log2) < row_bytes) p.zero_log2++;
@@ -665,7 +669,7 @@ TablePlan plan_table(const hf_embedding_backward_args &a, int cus) {
   p.order_at = take((size_t)a.ntokens * sizeof(uint2));
   p.other_at = take(p.passes > 1 ? (size_t)a.ntokens * sizeof(uint2) : 0);
   p.partial_at = take((size_t)p.nchunks * 2 * (size_t)p.slots * (size_t)p.vec * sizeof(float));
-  p.bytes = a.ntokens <= kFewTokens ? 0 : at;
+  p.bytes = at;
   return p;
 }
 
@@ -673,34 +677,34 @@ template <class T, class O, int VEC>
 hipError_t sum_tokens(const hf_embedding_backward_args &a, const TablePlan &p, const TableScratch &sc, int cus, hipStream_t s) {
   const unsigned long long sums = ((((unsigned long long)p.nchunks * p.col_tiles) << p.lanes_log2) + 255) / 256;
   const dim3 grid((unsigned)sums);
-  if (sums == 0) return hipSuccess;
-  if (p.lanes_log2 == 6)
-    hipLaunchKernelGGL((sum_rows_kernel<T, O, VEC, true>), grid, dim3(256), 0, s, a, sc, 6, p.col_tiles);
-  else
-    hipLaunchKernelGGL((sum_rows_kernel<T, O, VEC, false>), grid, dim3(256), 0, s, a, sc, p.lanes_log2, p.col_tiles);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.nchunks < 3) return e;   // a shared token crosses two chunk boundaries
-  const unsigned long long items = (unsigned long long)p.nchunks * p.col_tiles;
-  if (p.lanes_log2 == 6)
-    hipLaunchKernelGGL((join_rows_kernel<O, VEC, 16, true>), dim3((unsigned)std::min<unsigned long long>(items, (unsigned long long)cus * 4)), dim3(1024),
-                       0, s, a, sc, 6, p.col_tiles);
-  else
-    hipLaunchKernelGGL((join_rows_kernel<O, VEC, 4, false>), dim3((unsigned)std::min<unsigned long long>(items, (unsigned long long)cus * 16)), dim3(256),
-                       0, s, a, sc, p.lanes_log2, p.col_tiles);
+  const unsigned long long items = (unsigned long long)p.nchunks * p.col_tiles;   // of the join, at most
+  if constexpr (VEC > 1) {   // (rows of less than a slot are 8 lanes wide)
+    if (p.lanes_log2 == 6) {
+      hipLaunchKernelGGL((sum_rows_kernel<T, O, VEC, true>), grid, dim3(256), 0, s, a, sc, 6, p.col_tiles);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      hipLaunchKernelGGL((join_rows_kernel<O, VEC, 16, true>), dim3((unsigned)std::min<unsigned long long>(items, (unsigned long long)cus * 4)), dim3(1024),
+                         0, s, a, sc, 6, p.col_tiles);
+      return hipGetLastError();
+    }
+  }
+  hipLaunchKernelGGL((sum_rows_kernel<T, O, VEC, false>), grid, dim3(256), 0, s, a, sc, p.lanes_log2, p.col_tiles);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((join_rows_kernel<O, VEC, 4, false>), dim3((unsigned)std::min<unsigned long long>(items, (unsigned long long)cus * 16)), dim3(256),
+                     0, s, a, sc, p.lanes_log2, p.col_tiles);
   return hipGetLastError();
 }
 
-// `bytes`: of the table to a workgroup, all of which look through the tokens.
-template <class I, int WAVES, int KEYS>
-hipError_t sort_few(const hf_embedding_backward_args &a, const TablePlan &p, const TableScratch &sc, const ZeroRows &all, int64_t bytes,
-                    hipStream_t s) {
-  constexpr int64_t kThreads = 64 * WAVES;
-  int64_t rows = std::max<int64_t>(1, std::min<int64_t>(kThreads, bytes / (a.cols * (int64_t)all.element)));
+template <class I>
+hipError_t sort_few(const hf_embedding_backward_args &a, const TablePlan &p, const TableScratch &sc, const ZeroRows &all, hipStream_t s) {
+  constexpr int64_t kThreads = 64 * kSortFewWaves;
+  int64_t rows = std::max<int64_t>(1, std::min<int64_t>(kThreads, kSortFewBytes / (a.cols * (int64_t)all.element)));
   while (rows < kThreads && a.vocab / rows * kThreads >= (int64_t)1 << 31) rows = std::min(rows * 2, kThreads);   // a grid has less than 2^32 threads
   ZeroRows z = all;
   while (((int64_t)1 << z.lanes_log2) > kThreads) z.lanes_log2--;   // a workgroup's rows are its own
   const unsigned blocks = (unsigned)((a.vocab + rows - 1) / rows);
-  hipLaunchKernelGGL((sort_few_kernel<I, WAVES, KEYS>), dim3(1 + blocks), dim3(kThreads), 0, s, a, sc, p.passes, p.digit_bits, (unsigned)rows, z);
+  hipLaunchKernelGGL((sort_few_kernel<I>), dim3(1 + blocks), dim3(kThreads), 0, s, a, sc, p.passes, p.digit_bits, (unsigned)rows, z);
   return hipGetLastError();
 }
 
@@ -708,7 +712,7 @@ template <class I>
 hipError_t sort_tokens(const hf_embedding_backward_args &a, const TablePlan &p, const TableScratch &sc, const ZeroRows &all, hipStream_t s) {
   // One launch instead of two a digit: 24 against 30 us for 4096 tokens of a 2000 x 768 float32 table.  One workgroup's sort
   // of 4096 tokens (11 us) is only worth it next to a small table (50000 x 2048 bf16: 54 against 52 us).
-  if (a.ntokens <= 4096 && a.vocab * a.cols * (int64_t)all.element <= (int64_t)64 << 20) return sort_few<I, 8, 8>(a, p, sc, all, 65536, s);
+  if (a.ntokens <= kSortFewTokens && a.vocab * a.cols * (int64_t)all.element <= (int64_t)64 << 20) return sort_few<I>(a, p, sc, all, s);
   // the rows of zeros are shared evenly among the launches behind the first, which finds out what they are
   const unsigned parts = 2u * (unsigned)p.passes - 1u;
   ZeroRows z = {0, 0, all.lanes_log2, all.element};
@@ -723,16 +727,18 @@ hipError_t sort_tokens(const hf_embedding_backward_args &a, const TablePlan &p, 
   uint2 *in = nullptr, *out = p.passes % 2 ? sc.order : sc.other;
   for (int pass = 0; pass < p.passes; pass++) {
     const int shift = pass * p.digit_bits;
-    if (pass == 0)
-      hipLaunchKernelGGL((count_digits_kernel<I, true>), dim3(std::max(p.tiles, 1u)), dim3(kSortThreads), 0, s, a, sc, in, shift, p.digit_bits, z);
-    else if (const unsigned blocks = p.tiles + zero_blocks())
+    unsigned blocks = p.tiles;
+    if (pass == 0) {
+      hipLaunchKernelGGL((count_digits_kernel<I, true>), dim3(blocks), dim3(kSortThreads), 0, s, a, sc, in, shift, p.digit_bits, z);
+    } else {
+      blocks += zero_blocks();   // (sets z)
       hipLaunchKernelGGL((count_digits_kernel<I, false>), dim3(blocks), dim3(kSortThreads), 0, s, a, sc, in, shift, p.digit_bits, z);
-    if (const unsigned blocks = p.tiles + zero_blocks()) {
-      if (pass == 0)
-        hipLaunchKernelGGL((place_digits_kernel<I, true>), dim3(blocks), dim3(kSortThreads), 0, s, a, sc, in, out, shift, p.digit_bits, z);
-      else
-        hipLaunchKernelGGL((place_digits_kernel<I, false>), dim3(blocks), dim3(kSortThreads), 0, s, a, sc, in, out, shift, p.digit_bits, z);
     }
+    blocks = p.tiles + zero_blocks();
+    if (pass == 0)
+      hipLaunchKernelGGL((place_digits_kernel<I, true>), dim3(blocks), dim3(kSortThreads), 0, s, a, sc, in, out, shift, p.digit_bits, z);
+    else
+      hipLaunchKernelGGL((place_digits_kernel<I, false>), dim3(blocks), dim3(kSortThreads), 0, s, a, sc, in, out, shift, p.digit_bits, z);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     in = out;
