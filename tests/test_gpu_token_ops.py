@@ -325,6 +325,66 @@ def test_layer_norm_gradient_against_differences(cuda):
         check(got, want, 1e-5 * (1 + want.abs()), k)
 
 
+def shifted(pad, at):
+    """Rows cut out of wider ones: a row starts at element `at`, pad + cols elements behind the one before."""
+    def put(v):
+        buf = torch.full((v.shape[0], v.shape[1] + pad), float("nan"), device=v.device, dtype=v.dtype)
+        buf[:, at:at + v.shape[1]] = v
+        return buf[:, at:at + v.shape[1]]
+    return put
+
+
+# Every way rows of several waves are cut: two, three and four slots a lane, whole workgroups, rows that are read again, each
+# with a last slot that repeats elements and one that does not.
+WIDE_COLS = [4104, 4605, 7176, 7677, 9001, 12289, 12296, 14337, 16383, 16384, 16389, 24577, 30003, 32765, 32768, 32771, 40007]
+
+
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("cols", WIDE_COLS)
+def test_layer_norm_of_wide_rows(cuda, type, cols):
+    t = TYPES[type]
+    for rows, params, put in ((300 if cols < 8192 else 5, t, lambda v: v), (259 if cols < 8192 else 4, torch.float32, shifted(5, 3))):
+        x = rand((rows, cols), cols + rows, t, 2.0, 0.5)
+        w, b = rand((cols,), 1, params, 0.2, 1.0), rand((cols,), 2, params)
+        check_norm(x, w, b, 1e-5, run_norm(x, w, b, 1e-5, cuda, put), (type, cols, rows))
+
+
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("cols", WIDE_COLS)
+def test_layer_norm_backward_of_wide_rows(cuda, type, cols):
+    """Over more rows than there are workgroups where a workgroup takes several in turn."""
+    t = TYPES[type]
+    for rows, params, put in ((300 if cols <= 16384 else 131, t, lambda v: v), (5, torch.float32, shifted(3, 1))):
+        x, dy = rand((rows, cols), cols + rows, t, 2.0, 0.5), rand((rows, cols), cols, t, 0.1)
+        w, (mean, rstd) = rand((cols,), 1, params, 0.2, 1.0), stats(x)
+        check_grad(dy, x, mean, rstd, w, run_grad(dy, x, mean, rstd, w, cuda, put=put), (type, cols, rows))
+
+
+@pytest.mark.parametrize("rows, cols, type, params", [(8203, 1155, "f32", "f32"), (8200, 2056, "bf16", "bf16"), (9001, 4104, "f16", "f16"),
+                                                      (16411, 8192, "bf16", "f32"), (8300, 8200, "f32", "f32")])
+def test_layer_norm_over_several_rows_a_workgroup(cuda, rows, cols, type, params):
+    """Rows of several waves, each workgroup with several in turn; the last two are more than 256 MiB and read past the caches.
+    Bounds in 64 bits on the GPU, over the first, the last and every seventh row."""
+    t, p = TYPES[type], TYPES[params]
+    g = torch.Generator(device=cuda).manual_seed(rows)
+    x = (torch.randn((rows, cols), generator=g, device=cuda) * 2 + torch.randn((rows, 1), generator=g, device=cuda)).to(t)
+    w, b = (torch.randn((cols,), generator=g, device=cuda).to(p) for _ in range(2))
+    got = ops.run(ops.layer_norm(x, cols, w, b))
+    for part in (slice(0, 600), slice(rows - 600, rows), slice(0, rows, 7)):
+        check_norm(x[part], w, b, 1e-5, [v[part] for v in got], (rows, cols, part))
+
+
+def test_layer_norm_backward_past_the_caches(cuda):
+    """x and dy of more than 256 MiB; 64 bits on the GPU."""
+    rows, cols, t = 9001, 8192, torch.bfloat16
+    g = torch.Generator(device=cuda).manual_seed(9)
+    x, dy = (torch.randn((rows, cols), generator=g, device=cuda).to(t) for _ in range(2))
+    w = torch.randn((cols,), generator=g, device=cuda)
+    mean, rstd = stats(x)
+    got = ops.run(ops.layer_norm_backward(dy, x, cols, mean, rstd, w))
+    check_grad(dy, x, mean, rstd, w, got, "past the caches")
+
+
 # ------------------------------------------------------------------ embedding
 def ids(n, vocab, seed, bad=True):
     t = torch.randint(0, vocab, (n,), generator=gen(seed))
@@ -469,6 +529,21 @@ def test_embedding_backward_leaves_unused_rows_unread(cuda):
     (got,) = ops.run(ops.embedding_backward(dirty.to(cuda), tok.to(cuda), vocab, 1.0, 3))
     keep = torch.arange(vocab, device=cuda) != 9
     assert torch.equal(got[keep], clean[keep]) and torch.isinf(got[9]).all()
+
+
+@pytest.mark.parametrize("n, vocab, cols", [(500, 60, 40), (3000, 200, 40), (3000, 50000, 400), (6000, 200, 40)])
+def test_long_ids_are_no_short_ones(cuda, n, vocab, cols):
+    """Ids whose low word alone would name a row: the lookup and the gradient's three ways to sort them leave them out."""
+    tok = torch.randint(0, vocab, (n,), generator=gen(n))
+    tok[::3] += 1 << 32
+    tok[1::7] -= 1 << 32
+    tok[5], tok[6] = (1 << 63) - 1, -(1 << 63)
+    w, dy = rand((vocab, cols), 47), rand((n, cols), 48)
+    (out,) = ops.run(ops.embedding(tok.to(cuda), w.to(cuda)))
+    used = (tok >= 0) & (tok < vocab)
+    assert torch.equal(out.cpu(), torch.where(used[:, None], w[tok.clamp(0, vocab - 1)], torch.zeros(())))
+    check_table_grad(dy, tok, vocab, cuda, 1.0, None, None, (n, vocab))
+    check_table_grad(dy, tok, vocab, cuda, 1.0, int(tok[used][0]), None, (n, vocab, "pad"))
 
 
 def test_embedding_backward_strided_and_broadcast(cuda):
@@ -627,6 +702,40 @@ def test_graph_capture_and_replay(cuda):
         for got, want in zip(out, embed_and_norm(tok, table, w, b, 2.0, 5, dy)):
             assert torch.equal(got, want), i
         torch.cuda.synchronize()
+
+
+def test_kept_ops_captured_and_replayed(cuda):
+    """Ops that a program keeps, built before the capture, run eagerly, captured twice and replayed: each run reads what its
+    inputs hold then."""
+    n, vocab, cols = 3000, 700, 264
+    tok = torch.randint(0, vocab, (n,), generator=gen(92)).to(cuda)
+    table, w, dy = rand((vocab, cols), 93).to(cuda), rand((cols,), 94).to(cuda), rand((n, cols), 95).to(cuda)
+    look = ops.embedding(tok, table, 2.0)
+    norm = ops.layer_norm(look.outputs[0], cols, w)
+    norm_grad = ops.layer_norm_backward(dy, look.outputs[0], cols, *norm.outputs[1:], w)
+    kept = (look, norm, norm_grad, ops.embedding_backward(norm_grad.outputs[0], tok, vocab, 2.0))
+
+    def eager():
+        for op in kept:
+            ops.run(op)
+        torch.cuda.synchronize()
+        return [v.clone() for op in kept for v in op.outputs]
+    eager()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for g in graphs:
+        with torch.cuda.graph(g):
+            for op in kept:
+                ops.run(op)
+    for i in range(4):
+        tok.copy_(torch.randint(-1, vocab, (n,), generator=gen(96 + i)))
+        dy.copy_(rand((n, cols), 100 + i))
+        for op in kept:
+            for v in op.outputs:
+                v.fill_(7)
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        got = [v.clone() for op in kept for v in op.outputs]
+        assert all(torch.equal(a, b) for a, b in zip(got, eager())), i
 
 
 def test_two_graphs_and_a_side_stream(cuda):
