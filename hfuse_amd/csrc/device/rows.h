@@ -86,20 +86,36 @@ __device__ __forceinline__ int slot_repeats(int j, int cols) {
   return max(0, j * N - (cols - N));
 }
 
-// Sum over aligned groups of LANES lanes (a power of two up to 64), in every lane.  The steps inside 16 lanes are DPP moves
-// (quad permutes, mirrors of 8 and of 16: each pairs lanes whose partial sums cover disjoint halves, as an xor would).
+// Sum over aligned groups of LANES lanes (a power of two up to 64; FROM: already summed over groups of so many), in every
+// lane, of a float, of two side by side (their steps fill each other's waits) or, up to 16 lanes, of a double.  The steps inside 16 lanes are DPP moves (quad permutes, mirrors
+// of 8 and of 16: each pairs lanes whose partial sums cover disjoint halves, as an xor would).
+template <int CTRL>
+__device__ __forceinline__ int dpp_move(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false);
+}
 template <int CTRL>
 __device__ __forceinline__ float dpp_move(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+  return __builtin_bit_cast(float, dpp_move<CTRL>(__builtin_bit_cast(int, v)));
 }
-template <int LANES>
-__device__ __forceinline__ float lanes_sum(float v) {
-  if constexpr (LANES >= 2) v += dpp_move<0xB1>(v);    // quad_perm [1,0,3,2]
-  if constexpr (LANES >= 4) v += dpp_move<0x4E>(v);    // quad_perm [2,3,0,1]
-  if constexpr (LANES >= 8) v += dpp_move<0x141>(v);   // row_half_mirror
-  if constexpr (LANES >= 16) v += dpp_move<0x140>(v);  // row_mirror
-  if constexpr (LANES >= 32) v += __shfl_xor(v, 16);
-  if constexpr (LANES >= 64) v += __shfl_xor(v, 32);
+template <int CTRL>
+__device__ __forceinline__ float2 dpp_move(float2 v) {
+  return make_float2(dpp_move<CTRL>(v.x), dpp_move<CTRL>(v.y));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_move(double v) {
+  const int2 w = __builtin_bit_cast(int2, v);
+  return __builtin_bit_cast(double, make_int2(dpp_move<CTRL>(w.x), dpp_move<CTRL>(w.y)));
+}
+__device__ __forceinline__ float lane_xor(float v, int m) { return __shfl_xor(v, m); }
+__device__ __forceinline__ float2 lane_xor(float2 v, int m) { return make_float2(__shfl_xor(v.x, m), __shfl_xor(v.y, m)); }
+template <int LANES, int FROM = 1, class V>
+__device__ __forceinline__ V lanes_sum(V v) {
+  if constexpr (LANES >= 2 && FROM < 2) v += dpp_move<0xB1>(v);    // quad_perm [1,0,3,2]
+  if constexpr (LANES >= 4 && FROM < 4) v += dpp_move<0x4E>(v);    // quad_perm [2,3,0,1]
+  if constexpr (LANES >= 8) v += dpp_move<0x141>(v);               // row_half_mirror
+  if constexpr (LANES >= 16) v += dpp_move<0x140>(v);              // row_mirror
+  if constexpr (LANES >= 32) v += lane_xor(v, 16);
+  if constexpr (LANES >= 64) v += lane_xor(v, 32);
   return v;
 }
 

@@ -1,9 +1,10 @@
 // Token embedding, out[i] = scale W[t_i], and the gradient of the table, dW[v] = scale sum of dy[i] over i with t_i = v.
 //
 // Both are bound by HBM.  Measured on an MI355X with 131072 tokens and a table of 128000 x 4096 bf16, ids of a learnt
-// vocabulary (the k-th with a probability of about 1 / k): lookup 263 us (1.07 GB written, 0.67 GB fetched for 0.27 GB of
-// distinct rows: 6.3 TB/s); gradient 370-405 us for 2.1 GB = 5.2-5.7 TB/s, of which the sort and the rows of zeros beside
-// it take 135, the sums 225, the shared tokens 11.
+// vocabulary (the k-th with a probability of about 1 / k): lookup 264 us (1.07 GB written, 0.67 GB fetched for 0.27 GB of
+// distinct rows: 6.6 TB/s; 279 us a launch under the profiler); gradient, with the first id as padding, 370 us on the GPU and
+// 406 a call in a row of them for 2.06 GB = 5.1-5.6 TB/s: the sort and the rows of zeros beside it 134, the sums 225, the
+// shared tokens 11.
 #include <algorithm>
 
 #include "device/rows.h"

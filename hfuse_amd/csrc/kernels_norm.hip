@@ -1,11 +1,11 @@
 // Layer norm over the last dimension: mean = sum(x) / n, var = sum((x - mean)^2) / n, y = (x - mean) / sqrt(var + eps) w + b.
 //
 // Bound by HBM: a row is read once and written once, about 8 operations an element (2 a byte in 16 bits).  Measured on an
-// MI355X: 32768 x 8192 bf16 with float32 parameters 182 us = 5.9 TB/s (a copy of 2 GiB reaches 4.9 TB/s there), 3001 x 1155
-// float32 7.8 us, one row of 4096 bf16 2.4 us (an empty kernel takes 1.3).  The variance is the mean of squared
-// differences from the mean, not of squares, and where a row's sum is not exact the mean of the differences corrects both
-// (centred): rows with a large mean lose nothing.  Outputs are stored past the caches, and inputs read past
-// them where they cannot be there (past_caches): 203 -> 187 us.
+// MI355X: 32768 x 8192 bf16 with float32 parameters 184 us = 5.8 TB/s (196 a launch under the profiler; a copy of 2 GiB
+// reaches 4.9 TB/s there), 3001 x 1155 float32 8.2 us, one row of 4096 bf16 2.5 us (an empty kernel takes 1.3).  The variance
+// is the mean of squared differences from the mean, not of squares, and where a row's sum is not exact the mean of the
+// differences corrects both (centred): rows with a large mean lose nothing.  Outputs are stored past the caches, and
+// inputs read past them where they cannot be there (past_caches): 193 -> 185 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -21,9 +21,10 @@ namespace {
 // The sum of a row of 32-bit elements is rounded, so their differences d are taken from a number near the mean.  By how
 // much it is off is the mean of d, whose terms are as small as the row's spread: mean(x) = near + mean(d), and
 // var = mean(d^2) - mean(d)^2.  Of a constant row, d is a few units of x's last place, and their sum is exact.
-// 16-bit rows with a large mean have exact sums up to 2^16 (bf16) or 2^13 columns (f16): 8 or 11 bits an element and one for
-// every doubling make 24.  Their mean is rounded once, 2^-16 or 2^-13 of the elements' own step, and nothing is
-// corrected: the two operations an element would cost 184 -> 197 us at 32768 x 8192.
+// 16-bit rows with a large mean have exact sums of up to 2^16 (bf16) or 2^13 elements (f16): 8 or 11 bits an element and one
+// for every doubling make 24, and of f16 rows of more than 2^13 columns the sums of the waves are added in 64 bits.  Their
+// mean is rounded once, 2^-16 or 2^-13 of the elements' own step, and nothing is corrected: the two operations an element would
+// cost 184 -> 197 us at 32768 x 8192 bf16, and 360 -> 392 at 32768 x 16384 f16, where adding in 64 bits costs 360 -> 374.
 struct Centre {
   float shift, rstd;   // d - shift: the difference from the mean
 };
@@ -42,9 +43,10 @@ __device__ __forceinline__ Centre centred(float sum_d, float sum_d2, float n, fl
 template <class T, class P, int VEC, int VPT, int LANES, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_args a, int wide_lanes, bool stream) {
   constexpr bool kKeep = VPT <= 2 || BLOCK < 1024;   // weights and biases fit the registers next to two rows
-  // 32-bit rows, and f16 rows of more than 2^13 columns (two slots or more of 1024 threads)
-  constexpr bool kCentre = sizeof(T) == 4 || (std::is_same<T, f16_t>::value && VPT > 1 && BLOCK == 1024);
-  __shared__ float part[3][16];
+  constexpr bool kCentre = sizeof(T) == 4;
+  constexpr bool kWideJoin = std::is_same<T, f16_t>::value && VPT > 1 && BLOCK == 1024;   // f16 rows of more than 2^13 columns
+  __shared__ float part[16];
+  __shared__ float2 part2[16];
   const int lanes = LANES ? LANES : wide_lanes, groups = (int)blockDim.x / lanes;
   const int cols = (int)a.cols, t = (int)threadIdx.x % lanes, group = (int)threadIdx.x / lanes;
   const RowSlots<VEC, VPT> map(t, lanes, cols);
@@ -59,19 +61,19 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_ar
     for (int k = 0; k < VPT; k++) load_params(k, w[k], b[k]);
   }
   const float n = (float)cols, inv = 1.0f / n;
+  const double inv64 = kWideJoin ? 1.0 / (double)cols : 0.0;
   const int64_t step = (int64_t)gridDim.x * groups;
-  // Sums over a row.  The waves of a wide one, 16 at most, meet in LDS around a barrier: a slot is written again only behind
-  // the barrier of another.
-  auto leave = [&](float v, int which) {
-    v = lanes_sum<(LANES ? LANES : 64)>(v);
-    if (LANES == 0 && (threadIdx.x & 63u) == 0) part[which][threadIdx.x >> 6] = v;
-    return v;
+  // Sums over a row, of one value or two.  The waves of a wide one, 16 at most, leave theirs in LDS, and every lane has one of
+  // them behind the barrier.  A row has two sums in arrays of their own: each is written again only behind the other's barrier.
+  auto of_waves = [&](auto v, auto *part) {
+    if ((threadIdx.x & 63u) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    const int i = (int)threadIdx.x & 15, waves = lanes >> 6;
+    return i < waves ? part[group * waves + i] : decltype(v){};
   };
-  auto joined = [&](float v, int which) {
-    if constexpr (LANES == 0) {
-      const int i = (int)threadIdx.x & 15, waves = lanes >> 6;
-      v = lanes_sum<16>(i < waves ? part[which][group * waves + i] : 0.0f);
-    }
+  auto sum_row = [&](auto v, auto *part) {
+    v = lanes_sum<(LANES ? LANES : 64)>(v);
+    if constexpr (LANES == 0) v = lanes_sum<16>(of_waves(v, part));
     return v;
   };
   vec_t<T, VEC> next[VPT];
@@ -98,9 +100,13 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_ar
         for (int e = 0; e < VEC; e++) s += e >= map.skip[k] ? elem<T, VEC>(x[k], e) : 0.0f;
       }
     }
-    s = leave(s, 0);
-    if constexpr (LANES == 0) __syncthreads();
-    const float near = quotient(joined(s, 0), n, inv);
+    float near;
+    if constexpr (kWideJoin) {   // (a wave has 2^11 elements at most: four waves' sums are exact)
+      const float four = lanes_sum<4>(of_waves(lanes_sum<64>(s), part));
+      near = (float)(lanes_sum<16, 4>((double)four) * inv64);
+    } else {
+      near = quotient(sum_row(s, part), n, inv);
+    }
     s = 0.0f;
     float s2 = 0.0f, d[VPT][VEC];
 #pragma unroll
@@ -122,13 +128,13 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_ar
         }
       }
     }
-    s2 = leave(s2, 1);
-    if constexpr (kCentre) s = leave(s, 2);
-    if constexpr (LANES == 0) __syncthreads();
-    s2 = joined(s2, 1);
     Centre c = {0.0f, 0.0f};
-    if constexpr (kCentre) c = centred(joined(s, 2), s2, n, inv, a.eps);
-    else c.rstd = rsqrtf(s2 * inv + a.eps);
+    if constexpr (kCentre) {
+      const float2 sums = sum_row(make_float2(s, s2), part2);
+      c = centred(sums.x, sums.y, n, inv, a.eps);
+    } else {
+      c.rstd = rsqrtf(sum_row(s2, &part2[0].x) * inv + a.eps);
+    }
     if (row < a.rows) {
       T *y = static_cast<T *>(a.y) + row * a.y_stride;
 #pragma unroll
@@ -218,8 +224,8 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(hf_layer_norm_arg
 
 // Two rows a group of lanes in turn, if every CU has eight workgroups then: the second row is on its way while the first
 // is finished, and a workgroup is gone before its reads and writes fall into step with everyone's.  (65536 x 4096 bf16, trips
-// 1 / 2 / 3 / 4: 193 / 175 / 176 / 183 us.)  Float32 parameters next to 16-bit rows are as many bytes as two rows, and a
-// workgroup of 1024 is alone on half a CU: four (195 -> 186 us at 65536 x 4096, 207 -> 185 us at 16384 x 16384).
+// 1 / 2 / 3 / 4: 207 / 183 / 183 / 188 us.)  Float32 parameters next to 16-bit rows are as many bytes as two rows, and a
+// workgroup of 1024 is alone on half a CU: four (194 -> 187 us at 65536 x 4096, 209 -> 190 us at 16384 x 16384).
 template <class T, class P, int VEC, int VPT, int LANES, int BLOCK>
 hipError_t norm_rows(const hf_layer_norm_args &a, int lanes, int cus, hipStream_t s) {
   const int groups = std::max(1, 256 / lanes);
@@ -244,10 +250,10 @@ hipError_t norm_forward(const hf_layer_norm_args &a, int cus, hipStream_t s) {
   if (slots <= 64) return norm_rows<T, P, VEC, 1, 64, 256>(a, 64, cus, s);
   const int waves = (int)std::min<int64_t>((slots + 63) / 64, 65);   // wavefronts with one slot a lane
   // Fewer rows than CUs: a row's latency is all there is, and one slot a thread is the shortest (one row of 2048 / 4096 bf16
-  // 2.4 / 2.5 us, with two slots 2.8 / 2.7); with more rows it is slower (4096 x 1024: 7.9 us against 5.3).
+  // 2.3 / 2.5 us, with two slots 2.8 / 2.8); with more rows it is slower (4096 x 1024: 5.0 us against 4.5).
   if (a.rows <= cus && waves <= 16) return norm_rows<T, P, VEC, 1, 0, 1024>(a, waves * 64, cus, s);
-  // Two slots a lane (with four 8192 x 4096 bf16 takes 26.4 instead of 25.4 us, 65536 x 4096 177 instead of 175; with one
-  // 27.2 and 192), one or three where that leaves fewer lanes without a slot: their arithmetic costs the same.
+  // Two slots a lane (with four 8192 x 4096 bf16 takes 24.0 instead of 22.8 us, 65536 x 4096 180 instead of 184; with one
+  // 22.6 and 192), one or three where that leaves fewer lanes without a slot: their arithmetic costs the same.
   if (waves == 2) return norm_rows<T, P, VEC, 2, 64, 256>(a, 64, cus, s);
   if (waves == 3) return norm_rows<T, P, VEC, 3, 64, 256>(a, 64, cus, s);
   if (waves <= 16 && waves % 2 && waves % 3 == 0) return norm_rows<T, P, VEC, 3, 0, 512>(a, waves / 3 * 64, cus, s);

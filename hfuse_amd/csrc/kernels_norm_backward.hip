@@ -2,9 +2,10 @@
 //   dx = rstd (g - mean(g) - h mean(g h)),  dweight = sum over rows of dy h,  dbias = sum over rows of dy.
 //
 // Bound by HBM: x and dy are read once and dx is written once, about 14 operations an element.  Measured on an MI355X:
-// 32768 x 8192 bf16 274 us + 5 us for the sums of the parts = 5.8 TB/s, 5003 x 1155 f16 13.0 + 4.1 us, 64 x 1024 5.9 + 2.4.
-// The part draws so much power there that arithmetic costs time although it hides behind the memory: h and g formed twice
-// instead of kept in registers 320 us.
+// 32768 x 8192 bf16 274 us + 5 us for the sums of the parts = 5.8 TB/s, 5003 x 1155 f16 12.7 + 4.2 us, 64 x 1024 5.9 + 2.5;
+// 16384 x 8192 f32, whose rows take workgroups of 1024 that form h and g twice, 305 + 5 us = 5.2 TB/s.  The part draws so much
+// power there that arithmetic costs time although it hides behind the memory: h and g formed twice instead of kept in
+// registers 289 -> 395 us (32768 x 8192 bf16, many in turn).
 #include <algorithm>
 
 #include "device/rows.h"
@@ -19,8 +20,9 @@ namespace {
 // One pass over the rows: a group of lanes holds a row of x and of dy in registers, VPT slots of 16 bytes each, forms the
 // two sums over the row that dx needs, writes dx, and adds dy * h and dy to the 32-bit sums of its columns, which stay in
 // registers for all rows of the group.  The next row is on its way meanwhile.  A workgroup leaves one row of sums for
-// dweight and one for dbias in `parts`; sum_parts_kernel adds them up in an order of its own.  One workgroup a CU: two
-// write twice the parts and hold no more rows (150 registers a thread), 18 against 14 us at 5003 x 1155.  LANES: lanes to a
+// dweight and one for dbias in `parts`; sum_parts_kernel adds them up in an order of its own.  One workgroup a CU
+// (100 to 160 registers a thread, three or four waves a SIMD): two write twice the parts, 15.1 + 5.1 against 12.7 + 4.2 us at
+// 5003 x 1155 f16, 276 + 7.3 against 274 + 5.1 at 32768 x 8192 bf16, and win 0.6 of 19 us at 131072 x 128.  LANES: lanes to a
 // row, 0 for whole waves whose number the launch says.
 template <class T, class P, int VEC, int VPT, int LANES, int BLOCK, bool PARAMS>
 __global__ __launch_bounds__(BLOCK) void layer_norm_grad_kernel(hf_layer_norm_backward_args a, float *parts, int wide_lanes, bool stream) {
