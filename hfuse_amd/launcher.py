@@ -414,8 +414,8 @@ def _check_sizes(what: str, cols: int, rows: dict, params: dict = {}, stats: dic
     """rows: all of as many rows of `cols` elements as the first one has (or `count` says); params: cols elements; stats: one
     a row; None passes."""
     first, t = next(iter(rows.items()))
-    if cols <= 0 or t.numel() % cols:
-        raise ValueError(f"{what}: {first} of shape {tuple(t.shape)} is not made of rows of {cols}")
+    if cols <= 0 or (t is not None and t.numel() % cols):
+        raise ValueError(f"{what}: {first} is not made of rows of {cols}")
     n = t.numel() // cols if count < 0 else count
     for group, size in ((rows, n * cols), (params, cols), (stats, n)):
         for name, t in group.items():

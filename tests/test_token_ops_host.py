@@ -241,6 +241,19 @@ def test_argument_builders_take_other_shapes_of_the_same_sizes():
     assert (a.ntokens, a.vocab) == (0, 9)
 
 
+def test_argument_builders_pass_on_what_is_left_out():
+    """The library says what is missing; a list without outputs is enough for its workspace."""
+    a = H.layer_norm_args(rows(), None)
+    assert a.y is None and a.mean is None and (a.rows, a.cols) == (4, 6)
+    a = H.embedding_args(TOKENS, rows(n=9), None)
+    assert a.out is None and a.ntokens == 4
+    a = H.layer_norm_backward_args(rows(), rows(), None, None, dbias=LINE)
+    assert a.dx is None and a.mean is None and a.dbias == LINE.data_ptr()
+    for cols in (0, -1):
+        with pytest.raises(ValueError):
+            H.embedding_args(TOKENS, torch.zeros(9, 0), None) if cols == 0 else H.layer_norm_args(rows(), None, cols=cols)
+
+
 def test_argument_builders_take_the_types_of_the_header():
     for t, code in ((F32, L.HF_F32), (BF16, L.HF_BF16), (HALF, L.HF_F16)):
         for p in (t, F32):
