@@ -20,7 +20,8 @@ namespace {
 
 // The sum of a row of 32-bit elements is rounded, so their differences d are taken from a number near the mean.  By how
 // much it is off is the mean of d, whose terms are as small as the row's spread: mean(x) = near + mean(d), and
-// var = mean(d^2) - mean(d)^2.  Of a constant row, d is a few units of x's last place, and their sum is exact.
+// var = mean(d^2) - mean(d)^2.  Of a constant row, d is a few units of x's last place, and their sum is exact.  A row whose
+// mean is smaller than its spread needs none of it: the differences are rounded themselves, by as much as the sum was.
 // 16-bit rows with a large mean have exact sums of up to 2^16 (bf16) or 2^13 elements (f16): 8 or 11 bits an element and one
 // for every doubling make 24, and of f16 rows of more than 2^13 columns the sums of the waves are added in 64 bits.  Their
 // mean is rounded once, 2^-16 or 2^-13 of the elements' own step, and nothing is corrected: the two operations an element would
@@ -28,12 +29,12 @@ namespace {
 struct Centre {
   float shift, rstd;   // d - shift: the difference from the mean
 };
-__device__ __forceinline__ Centre centred(float sum_d, float sum_d2, float n, float inv, float eps) {
+__device__ __forceinline__ Centre centred(float near, float sum_d, float sum_d2, float n, float inv, float eps) {
   Centre c;
-  c.shift = quotient(sum_d, n, inv);
-  if (!(fabsf(c.shift) <= 3.402823466e38f)) c.shift = 0.0f;   // rows of infinities or NaN, or out of range: as they come
-  const float var = fmaf(-c.shift, c.shift, sum_d2 * inv);
-  c.rstd = rsqrtf((var < 0.0f ? 0.0f : var) + eps);           // (a NaN stays)
+  const float square = sum_d2 * inv;
+  c.shift = near * near > square ? quotient(sum_d, n, inv) : 0.0f;   // (nor do rows out of range, of infinities or of NaN)
+  const float var = fmaf(-c.shift, c.shift, square);
+  c.rstd = rsqrtf((var < 0.0f ? 0.0f : var) + eps);                  // (a NaN stays)
   return c;
 }
 
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_rows_kernel(hf_layer_norm_ar
     Centre c = {0.0f, 0.0f};
     if constexpr (kCentre) {
       const float2 sums = sum_row(make_float2(s, s2), part2);
-      c = centred(sums.x, sums.y, n, inv, a.eps);
+      c = centred(near, sums.x, sums.y, n, inv, a.eps);
     } else {
       c.rstd = rsqrtf(sum_row(s2, &part2[0].x) * inv + a.eps);
     }
@@ -203,7 +204,7 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(hf_layer_norm_arg
     leave(s, 1);
     leave(s2, 2);
     __syncthreads();
-    const Centre centre = centred(sum_of(1), sum_of(2), n, inv, a.eps);
+    const Centre centre = centred(near, sum_of(1), sum_of(2), n, inv, a.eps);
     T *y = static_cast<T *>(a.y) + row * a.y_stride;
     for (int j = tid; j < slots; j += 1024) {
       const int c = slot_column<VEC>(j, cols);

@@ -206,6 +206,23 @@ def test_layer_norm_of_rows_with_a_large_mean(cuda, type, cols):
         check(y, wy, ty + half(t) * (wy.abs() + ty) + floor(t), (type, cols, rows, "y"))
 
 
+@pytest.mark.parametrize("cols", [100, 1155, 4096, 8200, 20001])
+def test_layer_norm_mean_is_as_exact_as_one_sum(cuda, cols):
+    """A mean that is small beside the spread is the sum's, not corrected by the mean of the differences: those of one binade
+    are all rounded by the same last bits of the mean, up to U / 2 each, which does not average out.
+
+    Root mean square of the sum's own error: a partial sum of m terms of size 1 is about sqrt(m) and is rounded by a uniform
+    error of U sqrt(m / 3) at most, there are cols / m of them at each of the log2(cols) levels of a tree, which gives
+    U sqrt(cols / 3) a level, and the k terms a lane adds one after another count as k / 2 levels; with 2 levels for the quotient.
+    Half as much again for what is not independent, and the mean's rounding."""
+    x = rand((2000, cols), cols, torch.float32, 1.0, 0.02)
+    _, mean, _ = run_norm(x, None, None, 1e-5, cuda)
+    want = x.double().mean(1, keepdim=True)
+    rms = lambda e: float((e * e).mean().sqrt())
+    k = max(16, cols / 1024 + 4)
+    assert rms(mean.cpu().double() - want) <= 1.5 * U * math.sqrt((math.log2(cols) + k / 2 + 2) / (3 * cols)) + U * rms(want), cols
+
+
 def grad64(dy, x, mean, rstd, w):
     n, rows = x.shape[1], x.shape[0]
     dy, x, mean, rstd = dy.double(), x.double(), mean.double().view(-1, 1), rstd.double().view(-1, 1)
